@@ -45,8 +45,10 @@ typedef enum {
                                B2G_STATIC_SCRATCH_BYTES of workspace */
 } b2g_status;
 
-/* Weight element type (reference: FP16 kernels/gemv_fp16.cu, E4M3 kernels/gemv_fp8.cu). */
-enum { B2G_DTYPE_FP16 = 0, B2G_DTYPE_FP8_E4M3 = 1 };
+/* Element types (reference: FP16 kernels/gemv_fp16.cu, E4M3 kernels/gemv_fp8.cu).
+ * A GEMV's weights are FP16 or E4M3; BF16 is a type of the activations of the
+ * 8-bit integer product and of the attention operators further down. */
+enum { B2G_DTYPE_FP16 = 0, B2G_DTYPE_FP8_E4M3 = 1, B2G_DTYPE_BF16 = 2 };
 
 /* Scale modes.  NONE, TENSOR_FP16 and CHANNEL_FP16 are the reference's
  * ScaleMode {kScaleNone, kScaleTensor, kScaleChannel} (kernels/gemv_fp8.cu:459)
@@ -387,6 +389,180 @@ b2g_status b2g_stack_set_option(b2g_stack* st, int32_t key, int32_t value);
  * error).  tp_size > 1 is not handled here (see the Python TP driver). */
 b2g_status b2g_stack_enqueue(const b2g_stack* st, int32_t m, void* h, void* act,
                              void* workspace, b2g_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Matrix product in 8-bit integers with a scale for each row of x (token)
+ * and each output channel (no reference counterpart):
+ *   y[i, j] = epilogue(x_scales[i] * w_scales[j] * sum_k x_codes[i, k] * w_codes[j, k]).
+ * Any number of rows: the projections of a prompt chunk beside b2g_op's 1..8
+ * decode rows, with the same fusions.  The integer sum is exact; scales,
+ * SiLU and the residual are applied in fp32 and y is rounded once.
+ * ------------------------------------------------------------------------ */
+/* Row codes: v = x, or (rmsnorm) v = x * rsqrt(mean(x^2) + rms_eps) * gamma;
+ * scale = max(max|v|, 1e-12) / 127 and code = v / scale rounded to the nearest
+ * integer, ties to even, all in fp32.  A row with a NaN or an infinity gets
+ * the scale NaN and zero codes, so that every output of it is NaN.
+ * x: [m, ldx] FP16 or BF16, 16-byte aligned, ldx a multiple of 8;
+ * codes: [m, ld_codes] int8, 16-byte aligned, ld_codes a multiple of 16 (the
+ * bytes behind column k are not written); gamma: [k] of x's type or NULL (1). */
+typedef struct {
+  int32_t m, k;
+  int32_t dtype; /* B2G_DTYPE_FP16 or _BF16 */
+  int32_t rmsnorm;
+  const void* x;
+  int64_t ldx;
+  const void* gamma;
+  float rms_eps;
+  void* codes;
+  int64_t ld_codes;
+  float* scales; /* [m] */
+} b2g_i8_rows_args;
+b2g_status b2g_i8_quantize_rows(const b2g_i8_rows_args* args, b2g_stream_t stream);
+/* Weight codes by the same rule for each output channel; w16 is [K, N] (KN)
+ * or [N, K] (NK) of `dtype`, the codes are always [N, ld_codes] (K
+ * contiguous), which the product reads. */
+b2g_status b2g_i8_quantize_weights(const void* w16, int32_t K, int32_t N, int32_t layout, int32_t dtype,
+                                   void* codes, int64_t ld_codes, float* scales, b2g_stream_t stream);
+
+#define B2G_I8_MAX_K 131072 /* the int32 sum of this many products cannot overflow */
+typedef struct {
+  int32_t in_features;  /* K, 1..B2G_I8_MAX_K */
+  int32_t out_features; /* N (per weight plane) */
+  int32_t max_m;        /* rows per call */
+  int32_t dtype;        /* of x, residual, gamma and y: B2G_DTYPE_FP16 or _BF16 */
+  int32_t fuse;         /* B2G_FUSE_* mask; GATE_UP_SILU and RESIDUAL_ADD exclude each other */
+} b2g_i8_fields;
+typedef struct b2g_i8_op b2g_i8_op;
+typedef struct {
+  int32_t m;             /* 1..max_m */
+  const void* x;         /* [m, ldx] 16-bit rows to quantise, or NULL: */
+  int64_t ldx;
+  const void* gamma;     /* FUSE_RMSNORM_INPUT: [K] or NULL (1) */
+  float rms_eps;
+  const void* x_codes;   /* [m, ld_codes] int8 as b2g_i8_quantize_rows leaves them (x NULL) */
+  int64_t ld_codes;
+  const float* x_scales; /* [m] (x NULL) */
+  const void* w_codes;   /* [planes * N, ldw] int8: GATE_UP_SILU gate rows, then up rows;
+                            16-byte aligned, ldw a multiple of 16 */
+  int64_t ldw;
+  const float* w_scales; /* [planes * N] */
+  const void* residual;  /* [m, ldr], FUSE_RESIDUAL_ADD only (may alias y) */
+  int64_t ldr;
+  void* y;               /* [m, ldy] */
+  int64_t ldy;
+  void* workspace;       /* b2g_i8_workspace_size bytes, 256-byte aligned, zeroed once by
+                            b2g_i8_workspace_init; calls that can run at the same time
+                            need workspaces of their own */
+} b2g_i8_args;
+b2g_status b2g_i8_create(const b2g_i8_fields* fields, b2g_i8_op** out);
+b2g_status b2g_i8_destroy(b2g_i8_op* op);
+b2g_status b2g_i8_workspace_size(const b2g_i8_op* op, size_t* bytes);
+b2g_status b2g_i8_workspace_init(const b2g_i8_op* op, void* workspace, b2g_stream_t stream);
+/* Exactly one of x and x_codes; FUSE_RMSNORM_INPUT takes x. */
+b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* args, b2g_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Attention over a paged key/value cache (no reference counterpart): the
+ * append of new tokens with the position rotation, and the attention of the
+ * new tokens over everything cached.  Every length is read on the device, so
+ * a captured graph replays with other lengths in the same buffers.
+ *
+ * Cache: token `pos` of sequence b is row pos % page_size of page
+ * page_table[b][pos / page_size]; element (page, row, head, i) is at
+ * page * stride_page + row * stride_token + head * stride_head + i, which
+ * covers [pages, page_size, heads, dim] and [pages, heads, page_size, dim].
+ * The bases are 16-byte aligned and the strides multiples of 16 bytes.
+ * E4M3 caches hold value / scale[head] (scale NULL: 1), saturated.
+ * New tokens: the rows q_start[b] .. q_start[b + 1] - 1 belong to sequence
+ * b, whose last row is its token seq_lens[b] - 1 (seq_lens counts them);
+ * rows behind q_start[batch] are neither read nor written.
+ * A token whose page is not in 0..num_pages-1, or that lies past
+ * max_pages * page_size, is not written and not seen, and sets the device
+ * error word (b2g_device_error, code 6); a row before the start of its
+ * sequence (more new rows than seq_lens counts) is not written to the cache
+ * and sees nothing.
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  void* k;
+  void* v;
+  const float* k_scale; /* [kv_heads], E4M3 only, NULL = 1 */
+  const float* v_scale;
+  int64_t stride_page, stride_token, stride_head; /* elements, the same for k and v */
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype; /* the activations' type, or B2G_DTYPE_FP8_E4M3 */
+} b2g_kv_cache;
+typedef struct {
+  int32_t batch;             /* sequences */
+  int32_t rows;              /* rows of q, k, v and out (at least q_start[batch]) */
+  int32_t max_q;             /* most new tokens of one sequence: a hint that picks the
+                                kernel; any value gives the same results up to rounding */
+  int32_t max_pages;         /* entries of a page_table row */
+  int64_t page_table_stride; /* entries between rows */
+  const int32_t* q_start;    /* [batch + 1] */
+  const int32_t* seq_lens;   /* [batch] */
+  const int32_t* page_table; /* [batch, page_table_stride] */
+} b2g_kv_batch;
+
+/* kv_append: writes the new tokens' k (rotated) and v into their pages and,
+ * when q is given, the rotated q to q_out (may be q itself).  The rotation
+ * by pos * inv_freq[i] (angle in 64 bits) turns the pairs (i, i + rot/2), or
+ * (2i, 2i + 1) with `interleaved`, of the first rot = 2 * n_freq elements of
+ * a head; inv_freq NULL or n_freq 0: none.  Rows are [heads][head_dim] with
+ * the head's elements contiguous, 16-byte aligned, strides multiples of 8.
+ * The same token must not occur twice in one call. */
+typedef struct {
+  int32_t dtype;   /* of k, v, q: B2G_DTYPE_FP16 or _BF16 */
+  int32_t q_heads; /* 0 without q */
+  int32_t n_freq;  /* 0..head_dim / 2, a multiple of 8 */
+  int32_t interleaved;
+  const float* inv_freq;
+  const void* k;
+  int64_t stride_k, stride_k_head; /* elements between rows, heads */
+  const void* v;
+  int64_t stride_v, stride_v_head;
+  const void* q;
+  int64_t stride_q, stride_q_head;
+  void* q_out;
+  int64_t stride_qo, stride_qo_head;
+} b2g_kv_append_args;
+b2g_status b2g_kv_append(const b2g_kv_append_args* args, const b2g_kv_cache* cache, const b2g_kv_batch* batch,
+                         b2g_stream_t stream);
+
+/* Attention: for the row of token t of a sequence at position pos and head h,
+ *   out = sum_j softmax_j(scale * q . k[j, h / group]) v[j, h / group],
+ * over the cached tokens j <= pos, and j > pos - window if window > 0.
+ * fp32 scores, softmax statistics and sums; the probabilities are rounded to
+ * the activations' type for their product with v.  A row that sees nothing
+ * gives zeros and the log-sum -infinity. */
+typedef struct {
+  int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads, at most 32 times */
+  int32_t head_dim;          /* 64 or 128 */
+  int32_t max_batch;
+  int32_t dtype;             /* of q and out: B2G_DTYPE_FP16 or _BF16 */
+  int32_t cache_dtype;       /* dtype, or B2G_DTYPE_FP8_E4M3 */
+} b2g_attn_fields;
+typedef struct b2g_attn b2g_attn;
+typedef struct {
+  const void* q;
+  int64_t stride_q, stride_q_head;
+  void* out;
+  int64_t stride_o, stride_o_head;
+  float* lse; /* [rows, q_heads] natural log of the sum of exp(scale * q . k), or NULL */
+  float scale;
+  int32_t window; /* 0 = none */
+  void* workspace; /* b2g_attn_workspace_size bytes, 256-byte aligned, zeroed once by
+                      b2g_attn_workspace_init; calls that can run at the same time need
+                      workspaces of their own */
+} b2g_attn_args;
+b2g_status b2g_attn_create(const b2g_attn_fields* fields, b2g_attn** out);
+b2g_status b2g_attn_destroy(b2g_attn* op);
+b2g_status b2g_attn_workspace_size(const b2g_attn* op, size_t* bytes);
+b2g_status b2g_attn_workspace_init(const b2g_attn* op, void* workspace, b2g_stream_t stream);
+b2g_status b2g_attn_enqueue(const b2g_attn* op, const b2g_attn_args* args, const b2g_kv_cache* cache,
+                            const b2g_kv_batch* batch, b2g_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,7 @@ LIB_PATH = HERE / "libb200gemv.so"
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_PEER_TIMEOUT, ERR_OOM, ERR_DEVICE, ERR_SCRATCH_LIMIT = range(8)
 STATIC_SCRATCH_BYTES = 2 * 1024 * 1024  # B2G_STATIC_SCRATCH_BYTES
-DTYPE = {"fp16": 0, "fp8_e4m3": 1}
+DTYPE = {"fp16": 0, "fp8_e4m3": 1, "bf16": 2, "e4m3": 1}
 SCALE = {"none": 0, "tensor_fp16": 1, "channel_fp16": 2, "channel_fp32": 3}
 LAYOUT = {"KN": 0, "NK": 1}
 FUSE_NONE, FUSE_GATE_UP_SILU, FUSE_RMSNORM_INPUT, FUSE_RESIDUAL_ADD = 0, 1, 2, 4
@@ -85,6 +85,58 @@ class TpComm(ctypes.Structure):
                 ("counters", ctypes.c_void_p * TP_MAX_RANKS), ("epoch", ctypes.c_void_p)]
 
 
+class I8RowsArgs(ctypes.Structure):
+    _fields_ = [("m", ctypes.c_int32), ("k", ctypes.c_int32), ("dtype", ctypes.c_int32), ("rmsnorm", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("gamma", ctypes.c_void_p),
+                ("rms_eps", ctypes.c_float), ("codes", ctypes.c_void_p), ("ld_codes", ctypes.c_int64),
+                ("scales", ctypes.c_void_p)]
+
+
+class I8Fields(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("in_features", "out_features", "max_m", "dtype", "fuse")]
+
+
+class I8Args(ctypes.Structure):
+    _fields_ = [("m", ctypes.c_int32), ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("gamma", ctypes.c_void_p),
+                ("rms_eps", ctypes.c_float), ("x_codes", ctypes.c_void_p), ("ld_codes", ctypes.c_int64),
+                ("x_scales", ctypes.c_void_p), ("w_codes", ctypes.c_void_p), ("ldw", ctypes.c_int64),
+                ("w_scales", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_int64),
+                ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("workspace", ctypes.c_void_p)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("stride_page", ctypes.c_int64), ("stride_token", ctypes.c_int64),
+                ("stride_head", ctypes.c_int64), ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_q", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("page_table_stride", ctypes.c_int64), ("q_start", ctypes.c_void_p),
+                ("seq_lens", ctypes.c_void_p), ("page_table", ctypes.c_void_p)]
+
+
+class KvAppendArgs(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("n_freq", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("inv_freq", ctypes.c_void_p),
+                ("k", ctypes.c_void_p), ("stride_k", ctypes.c_int64), ("stride_k_head", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("stride_v", ctypes.c_int64), ("stride_v_head", ctypes.c_int64),
+                ("q", ctypes.c_void_p), ("stride_q", ctypes.c_int64), ("stride_q_head", ctypes.c_int64),
+                ("q_out", ctypes.c_void_p), ("stride_qo", ctypes.c_int64), ("stride_qo_head", ctypes.c_int64)]
+
+
+class AttnFields(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("q_heads", "kv_heads", "head_dim", "max_batch", "dtype", "cache_dtype")]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("stride_q", ctypes.c_int64), ("stride_q_head", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("stride_o", ctypes.c_int64), ("stride_o_head", ctypes.c_int64),
+                ("lse", ctypes.c_void_p), ("scale", ctypes.c_float), ("window", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p)]
+
+
 # Every exported entry point and its ctypes signature (kept in step with
 # include/b200gemv.h; the tests check the two agree).
 _P, _I32, _I64, _SZ = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
@@ -123,6 +175,21 @@ SIGNATURES = {
     "b2g_stack_workspace_size": ([_P, _I32, ctypes.POINTER(_SZ)], ctypes.c_int),
     "b2g_stack_workspace_init": ([_P, _P, _P], ctypes.c_int),
     "b2g_stack_enqueue": ([_P, _I32, _P, _P, _P, _P], ctypes.c_int),
+    "b2g_i8_quantize_rows": ([ctypes.POINTER(I8RowsArgs), _P], ctypes.c_int),
+    "b2g_i8_quantize_weights": ([_P, _I32, _I32, _I32, _I32, _P, _I64, _P, _P], ctypes.c_int),
+    "b2g_i8_create": ([ctypes.POINTER(I8Fields), ctypes.POINTER(_P)], ctypes.c_int),
+    "b2g_i8_destroy": ([_P], ctypes.c_int),
+    "b2g_i8_workspace_size": ([_P, ctypes.POINTER(_SZ)], ctypes.c_int),
+    "b2g_i8_workspace_init": ([_P, _P, _P], ctypes.c_int),
+    "b2g_i8_enqueue": ([_P, ctypes.POINTER(I8Args), _P], ctypes.c_int),
+    "b2g_kv_append": ([ctypes.POINTER(KvAppendArgs), ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), _P],
+                      ctypes.c_int),
+    "b2g_attn_create": ([ctypes.POINTER(AttnFields), ctypes.POINTER(_P)], ctypes.c_int),
+    "b2g_attn_destroy": ([_P], ctypes.c_int),
+    "b2g_attn_workspace_size": ([_P, ctypes.POINTER(_SZ)], ctypes.c_int),
+    "b2g_attn_workspace_init": ([_P, _P, _P], ctypes.c_int),
+    "b2g_attn_enqueue": ([_P, ctypes.POINTER(AttnArgs), ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), _P],
+                         ctypes.c_int),
 }
 
 _lib = None
@@ -427,3 +494,331 @@ def tp_gather(comm, buf: int, push_op, h, stream=None):
     check(lib().b2g_tp_gather(ctypes.byref(comm), buf, push_op.h, h.shape[0], ctypes.c_void_p(h.data_ptr()),
                               _rows_stride(h), _stream(stream)), "b2g_tp_gather")
     return h
+
+
+# ---------------------------------------------------------------------------
+# 8-bit integer product, paged cache, attention
+# ---------------------------------------------------------------------------
+def _act_code(t):
+    """B2G_DTYPE_* of 16-bit activations."""
+    import torch
+    if t.dtype == torch.float16:
+        return 0
+    if t.dtype == torch.bfloat16:
+        return 2
+    raise ValueError(f"expected float16 or bfloat16, got {t.dtype}")
+
+
+def _act_type(code):
+    import torch
+    return {0: torch.float16, 2: torch.bfloat16}[code]
+
+
+def _on(device, *tensors):
+    """The current device holds every tensor (the library launches there)."""
+    import torch
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+
+
+def _matrix(t, dtype, rows, cols, what):
+    if t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: expected [{rows}, {cols}] {dtype} with contiguous rows, got {tuple(t.shape)} "
+                         f"{t.dtype} strides {t.stride()}")
+
+
+def _ld(t, align):
+    """Row stride in elements; a single row may carry any, so it gets an aligned one."""
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // align) * align
+
+
+def _vector(t, dtype, n, what):
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: expected {n} contiguous {dtype}, got {tuple(t.shape)} {t.dtype}")
+
+
+class _Made:
+    """Buffers that a call makes for itself on `stream`: made under that
+    stream, so the allocator does not hand them on before its work is done."""
+
+    def __init__(self, stream):
+        import torch
+        self.ctx = None if stream is None else torch.cuda.stream(stream)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *a):
+        if self.ctx is not None:
+            self.ctx.__exit__(*a)
+
+
+def _codes(rows, cols, device):
+    """[rows, cols] int8 whose rows start 16-byte aligned, as the product reads them."""
+    import torch
+    return torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=device)[:, :cols]
+
+
+def quantize_i8_rows(x, gamma=None, rms_eps=None, codes=None, scales=None, stream=None):
+    """Codes [m, k] int8 and scales [m] fp32 of 16-bit rows (b2g_i8_quantize_rows).
+
+    With rms_eps the rows are RMS-normalised first (times gamma, if given).
+    """
+    import torch
+    m, k = x.shape
+    _on(x.device, x, gamma, codes, scales)
+    _matrix(x, x.dtype, m, k, "x")
+    if gamma is not None:
+        _vector(gamma, x.dtype, k, "gamma")
+    with _Made(stream):
+        if codes is None:
+            codes = _codes(m, k, x.device)
+        if scales is None:
+            scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    _matrix(codes, torch.int8, m, k, "codes")
+    _vector(scales, torch.float32, m, "scales")
+    a = I8RowsArgs(m, k, _act_code(x), rms_eps is not None, x.data_ptr(), _ld(x, 8),
+                   None if gamma is None else gamma.data_ptr(), rms_eps or 0.0, codes.data_ptr(), _ld(codes, 16),
+                   scales.data_ptr())
+    check(lib().b2g_i8_quantize_rows(ctypes.byref(a), _stream(stream)), "b2g_i8_quantize_rows")
+    return codes, scales
+
+
+def quantize_i8_weights(w16, layout="KN", stream=None):
+    """Codes [N, K] int8 and scales [N] fp32 of 16-bit weights [K, N] (KN) or [N, K] (NK)."""
+    import torch
+    lay = _code(LAYOUT, layout)
+    K, N = (w16.shape if lay == 0 else w16.shape[::-1])
+    _on(w16.device, w16)
+    if not w16.is_contiguous():
+        raise ValueError("w16 must be contiguous")
+    with _Made(stream):
+        codes = _codes(N, K, w16.device)
+        scales = torch.empty(N, dtype=torch.float32, device=w16.device)
+    check(lib().b2g_i8_quantize_weights(_ptr(w16), K, N, lay, _act_code(w16), _ptr(codes), _ld(codes, 16),
+                                        _ptr(scales), _stream(stream)), "b2g_i8_quantize_weights")
+    return codes, scales
+
+
+class I8Op:
+    """y[m, N] = epilogue(sx[m] * sw[N] * (x codes [m, K] . w codes [N, K])), any m up to max_m.
+
+    The fusions are GemvOp's: FUSE_RMSNORM_INPUT (rows normalised before they
+    are quantised), FUSE_GATE_UP_SILU (w holds the gate rows, then the up
+    rows: [2N, K]), FUSE_RESIDUAL_ADD.
+    """
+
+    def __init__(self, in_features: int, out_features: int, max_m: int, fuse: int = FUSE_NONE, dtype="fp16"):
+        self.K, self.N, self.max_m, self.fuse = in_features, out_features, max_m, fuse
+        self.dtype = _code(DTYPE, dtype)
+        self.planes = 2 if fuse & FUSE_GATE_UP_SILU else 1
+        h = ctypes.c_void_p()
+        f = I8Fields(in_features, out_features, max_m, self.dtype, fuse)
+        check(lib().b2g_i8_create(ctypes.byref(f), ctypes.byref(h)), "b2g_i8_create")
+        self.h = h
+        self._type = _act_type(self.dtype)
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.b2g_i8_destroy(self.h)
+            self.h = None
+
+    def workspace_bytes(self) -> int:
+        n = ctypes.c_size_t()
+        check(lib().b2g_i8_workspace_size(self.h, ctypes.byref(n)), "b2g_i8_workspace_size")
+        return n.value
+
+    def workspace(self, device="cuda", stream=None):
+        """A zeroed workspace.  Calls that can overlap (other streams, graphs
+        replayed at the same time) need one each."""
+        import torch
+        with _Made(stream):
+            ws = torch.empty(self.workspace_bytes(), dtype=torch.uint8, device=device)
+        check(lib().b2g_i8_workspace_init(self.h, _ptr(ws), _stream(stream)), "b2g_i8_workspace_init")
+        return ws
+
+    def _enqueue(self, m, x, gamma, rms_eps, codes, scales, wq, sw, residual, y, workspace, stream):
+        import torch
+        first = x if codes is None else codes
+        _on(first.device, gamma, scales, wq, sw, residual, y, workspace)
+        _matrix(wq, torch.int8, self.planes * self.N, self.K, "wq")
+        _vector(sw, torch.float32, self.planes * self.N, "sw")
+        if residual is not None:
+            _matrix(residual, self._type, m, self.N, "residual")
+        if y is None:
+            with _Made(stream):
+                y = torch.empty((m, self.N), dtype=self._type, device=first.device)
+        else:
+            _matrix(y, self._type, m, self.N, "y")
+        if workspace is None:
+            workspace = self.workspace(first.device, stream)
+        elif workspace.numel() * workspace.element_size() < self.workspace_bytes() or not workspace.is_contiguous():
+            raise ValueError(f"the workspace needs {self.workspace_bytes()} contiguous bytes")
+        a = I8Args(m, None if x is None else x.data_ptr(), 0 if x is None else _ld(x, 8),
+                   None if gamma is None else gamma.data_ptr(), rms_eps,
+                   None if codes is None else codes.data_ptr(), 0 if codes is None else _ld(codes, 16),
+                   None if scales is None else scales.data_ptr(), wq.data_ptr(), _ld(wq, 16), sw.data_ptr(),
+                   None if residual is None else residual.data_ptr(), 0 if residual is None else _ld(residual, 1),
+                   y.data_ptr(), _ld(y, 1), workspace.data_ptr())
+        check(lib().b2g_i8_enqueue(self.h, ctypes.byref(a), _stream(stream)), "b2g_i8_enqueue")
+        return y
+
+    def enqueue(self, x, wq, sw, y=None, workspace=None, residual=None, gamma=None, rms_eps: float = 1e-5,
+                stream=None):
+        """y of 16-bit rows x [m, K], quantised (and normalised) on the way."""
+        _matrix(x, self._type, x.shape[0], self.K, "x")
+        if gamma is not None:
+            _vector(gamma, self._type, self.K, "gamma")
+        return self._enqueue(x.shape[0], x, gamma, rms_eps, None, None, wq, sw, residual, y, workspace, stream)
+
+    def enqueue_codes(self, xq, sx, wq, sw, y=None, workspace=None, residual=None, stream=None):
+        """y of rows that quantize_i8_rows has quantised (one quantisation, several products)."""
+        import torch
+        _matrix(xq, torch.int8, xq.shape[0], self.K, "xq")
+        _vector(sx, torch.float32, xq.shape[0], "sx")
+        return self._enqueue(xq.shape[0], None, None, 0.0, xq, sx, wq, sw, residual, y, workspace, stream)
+
+
+class PagedCache:
+    """A paged key/value cache over two tensors of one shape and strides:
+    [pages, page_size, heads, dim] (layout "NHD") or [pages, heads, page_size,
+    dim] ("HND"), float16, bfloat16 or float8_e4m3fn.  An 8-bit cache holds
+    value / scale[head] (k_scale, v_scale: [heads] float32, None = 1)."""
+
+    def __init__(self, k, v, layout="NHD", k_scale=None, v_scale=None):
+        import torch
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("k and v: two 4-d tensors of one shape, type and strides, the last axis contiguous")
+        code = {torch.float16: 0, torch.bfloat16: 2, torch.float8_e4m3fn: 1}.get(k.dtype)
+        if code is None or layout not in ("NHD", "HND"):
+            raise ValueError(f"cache type {k.dtype}, layout {layout}")
+        tok, head = (1, 2) if layout == "NHD" else (2, 1)
+        for s in (k_scale, v_scale):
+            if s is not None:
+                _vector(s, torch.float32, k.shape[head], "k_scale, v_scale")
+        if any(t is not None and t.device != k.device for t in (v, k_scale, v_scale)):
+            raise ValueError("the cache's tensors are on different devices")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.page_size, self.kv_heads, self.head_dim, self.dtype = k.shape[tok], k.shape[head], k.shape[3], code
+        self.c = KvCache(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
+                         None if v_scale is None else v_scale.data_ptr(), k.stride(0), k.stride(tok),
+                         k.stride(head), k.shape[0], self.page_size, self.kv_heads, self.head_dim, code)
+
+
+def _kv_batch(device, rows, q_start, seq_lens, page_table, max_q):
+    import torch
+    batch = seq_lens.shape[0]
+    _on(device, q_start, seq_lens, page_table)
+    _vector(q_start, torch.int32, batch + 1, "q_start")
+    _vector(seq_lens, torch.int32, batch, "seq_lens")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or \
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"page_table: expected [{batch}, pages] int32 with contiguous rows")
+    return KvBatch(batch, rows, max_q or rows, page_table.shape[1], _ld(page_table, 1), q_start.data_ptr(),
+                   seq_lens.data_ptr(), page_table.data_ptr())
+
+
+def _heads(t, rows, heads, dim, dtype, what):
+    if t.dtype != dtype or t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != dim or \
+            t.stride(2) != 1:
+        raise ValueError(f"{what}: expected [{rows}, {heads}, {dim}] {dtype} with a contiguous last axis, got "
+                         f"{tuple(t.shape)} {t.dtype} strides {t.stride()}")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def kv_append(k, v, cache, q_start, seq_lens, page_table, q=None, q_out=None, inv_freq=None,
+              interleaved: bool = False, stream=None):
+    """Writes the new tokens' k (rotated) and v [rows, kv_heads, dim] into the
+    cache's pages, and the rotated q to q_out (default: q itself); b2g_kv_append.
+
+    q_start [batch + 1], seq_lens [batch] (new tokens counted) and page_table
+    [batch, pages] are int32.  inv_freq [n] float32 turns the first 2n elements
+    of a head by pos * inv_freq (None: no rotation).
+    """
+    import torch
+    rows, dim = k.shape[0], cache.head_dim
+    _on(k.device, v, cache.k, q, q_out, inv_freq)
+    b = _kv_batch(k.device, rows, q_start, seq_lens, page_table, 0)
+    kk = _heads(k, rows, cache.kv_heads, dim, k.dtype, "k")
+    vv = _heads(v, rows, cache.kv_heads, dim, k.dtype, "v")
+    qq = qo = (None, 0, 0)
+    if q is not None:
+        qq = _heads(q, rows, q.shape[1], dim, k.dtype, "q")
+        qo = qq if q_out is None else _heads(q_out, rows, q.shape[1], dim, k.dtype, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if inv_freq is not None:
+        _vector(inv_freq, torch.float32, inv_freq.shape[0], "inv_freq")
+    a = KvAppendArgs(_act_code(k), 0 if q is None else q.shape[1], 0 if inv_freq is None else inv_freq.shape[0],
+                     1 if interleaved else 0, None if inv_freq is None else inv_freq.data_ptr(), *kk, *vv, *qq, *qo)
+    check(lib().b2g_kv_append(ctypes.byref(a), ctypes.byref(cache.c), ctypes.byref(b), _stream(stream)),
+          "b2g_kv_append")
+    return q if q_out is None else q_out
+
+
+class AttnOp:
+    """Attention of new tokens over a PagedCache (b2g_attn_enqueue): one token
+    of a decode step or a chunk of a prompt, ragged over the batch."""
+
+    def __init__(self, q_heads: int, kv_heads: int, head_dim: int, max_batch: int, dtype="fp16", cache_dtype=None):
+        self.q_heads, self.kv_heads, self.head_dim, self.max_batch = q_heads, kv_heads, head_dim, max_batch
+        self.dtype = _code(DTYPE, dtype)
+        self.cache_dtype = self.dtype if cache_dtype is None else _code(DTYPE, cache_dtype)
+        h = ctypes.c_void_p()
+        f = AttnFields(q_heads, kv_heads, head_dim, max_batch, self.dtype, self.cache_dtype)
+        check(lib().b2g_attn_create(ctypes.byref(f), ctypes.byref(h)), "b2g_attn_create")
+        self.h = h
+        self._type = _act_type(self.dtype)
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.b2g_attn_destroy(self.h)
+            self.h = None
+
+    def workspace_bytes(self) -> int:
+        n = ctypes.c_size_t()
+        check(lib().b2g_attn_workspace_size(self.h, ctypes.byref(n)), "b2g_attn_workspace_size")
+        return n.value
+
+    def workspace(self, device="cuda", stream=None):
+        """A zeroed workspace.  Calls that can overlap (other streams, graphs
+        replayed at the same time) need one each."""
+        import torch
+        with _Made(stream):
+            ws = torch.empty(self.workspace_bytes(), dtype=torch.uint8, device=device)
+        check(lib().b2g_attn_workspace_init(self.h, _ptr(ws), _stream(stream)), "b2g_attn_workspace_init")
+        return ws
+
+    def enqueue(self, q, cache, q_start, seq_lens, page_table, max_q=None, scale=None, window: int = 0, out=None,
+                lse=None, workspace=None, stream=None):
+        """out [rows, q_heads, dim] of q; lse [rows, q_heads] float32 receives the log-sums.
+
+        max_q: the most new tokens of one sequence (None: unknown), a hint that
+        picks the kernel.  scale: default 1 / sqrt(dim).  window: a token sees
+        the last `window` positions, its own among them (0: all).
+        """
+        import torch
+        rows = q.shape[0]
+        _on(q.device, cache.k, out, lse, workspace)
+        b = _kv_batch(q.device, rows, q_start, seq_lens, page_table, max_q)
+        qq = _heads(q, rows, self.q_heads, self.head_dim, self._type, "q")
+        if out is None:
+            with _Made(stream):
+                out = torch.empty((rows, self.q_heads, self.head_dim), dtype=self._type, device=q.device)
+        oo = _heads(out, rows, self.q_heads, self.head_dim, self._type, "out")
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (rows, self.q_heads) or
+                                not lse.is_contiguous()):
+            raise ValueError(f"lse: expected [{rows}, {self.q_heads}] contiguous float32")
+        if workspace is None:
+            workspace = self.workspace(q.device, stream)
+        elif workspace.numel() * workspace.element_size() < self.workspace_bytes() or not workspace.is_contiguous():
+            raise ValueError(f"the workspace needs {self.workspace_bytes()} contiguous bytes")
+        a = AttnArgs(*qq, *oo, None if lse is None else lse.data_ptr(),
+                     self.head_dim ** -0.5 if scale is None else scale, window, workspace.data_ptr())
+        check(lib().b2g_attn_enqueue(self.h, ctypes.byref(a), ctypes.byref(cache.c), ctypes.byref(b),
+                                     _stream(stream)), "b2g_attn_enqueue")
+        return out

@@ -15,8 +15,9 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libb200gemv.so"
-SOURCES = ["gemv.cu", "pack.cu", "static_scratch.cu", "api.cpp"]
-HEADERS = ["device.cuh", "gemv.h"]
+SOURCES = ["gemv.cu", "pack.cu", "static_scratch.cu", "i8.cu", "kv_append.cu", "attention.cu", "api.cpp",
+           "serve_api.cpp"]
+HEADERS = ["device.cuh", "gemv.h", "serve.h", "serve.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -17,6 +17,7 @@
 
 #include "../../include/b200gemv.h"
 #include "gemv.h"
+#include "serve.h"
 
 using namespace b2g;
 
@@ -269,6 +270,17 @@ void fill_plan(const b2g_op* op, int m, const LaunchPlan& lp, void* workspace, i
 }
 
 }  // namespace
+
+namespace b2g {
+
+int* registered_error_word(int dev) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (dev < 0 || dev >= 64) return nullptr;
+  if (!g_err_word[dev]) g_err_word[dev] = device_error_word();
+  return g_err_word[dev];
+}
+
+}  // namespace b2g
 
 extern "C" {
 

@@ -1,0 +1,69 @@
+// serve.h -- internal interface between the host API (serve_api.cpp) and the
+// kernels of the 8-bit integer product (i8.cu), the cache append
+// (kv_append.cu) and the attention over the cache (attention.cu).
+#pragma once
+#include <cstddef>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "../../include/b200gemv.h"
+
+namespace b2g {
+
+// api.cpp: this device's error word, registered so that b2g_device_error
+// finds it (NULL: no such device, or a CUDA error).
+int* registered_error_word(int dev);
+
+// ---------------------------------------------------------------------------
+// i8.cu
+// ---------------------------------------------------------------------------
+struct I8RowsParams {
+  const void* x;
+  long long ldx;
+  const void* gamma;
+  float eps;
+  int8_t* codes;
+  long long ldc;
+  float* scales;
+  int m, k, bf16, rmsnorm;
+};
+cudaError_t launch_i8_quantize_rows(const I8RowsParams& p, cudaStream_t stream);
+cudaError_t launch_i8_quantize_weights(const void* w, int K, int N, int layout, int bf16, int8_t* codes,
+                                       long long ldc, float* scales, cudaStream_t stream);
+
+struct I8Params {
+  const int8_t* x;  // [m, ldx] codes
+  long long ldx;
+  const float* sx;
+  const int8_t* w;  // [planes * n, ldw] codes
+  long long ldw;
+  const float* sw;
+  const void* residual;
+  long long ldr;
+  void* y;
+  long long ldy;
+  int m, n, k, planes, bf16;
+};
+cudaError_t launch_i8_product(const I8Params& p, cudaStream_t stream);
+
+// ---------------------------------------------------------------------------
+// kv_append.cu, attention.cu
+// ---------------------------------------------------------------------------
+struct KvAppendParams {
+  b2g_kv_append_args a;
+  b2g_kv_cache c;
+  b2g_kv_batch b;
+  int* error;
+};
+cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t stream);
+
+struct AttnParams {
+  b2g_attn_args a;
+  b2g_kv_cache c;
+  b2g_kv_batch b;
+  int q_heads, group, bf16;
+  int* error;
+};
+cudaError_t launch_attention(const AttnParams& p, cudaStream_t stream);
+
+}  // namespace b2g
