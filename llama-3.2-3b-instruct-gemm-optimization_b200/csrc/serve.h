@@ -44,7 +44,12 @@ struct I8Params {
   long long ldy;
   int m, n, k, planes, bf16;
 };
-cudaError_t launch_i8_product(const I8Params& p, cudaStream_t stream);
+// Bytes of the split tiles' partial sums for calls of up to max_m rows.
+size_t i8_partial_bytes(int max_m, int planes, int num_sms);
+// counters: [num_sms] zeros, left zero.  pdl: the launch before this one in
+// the stream is the quantiser of p.x (the weights may be read before it ends).
+cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int* partials, int* error, bool pdl,
+                              cudaStream_t stream);
 
 // ---------------------------------------------------------------------------
 // kv_append.cu, attention.cu

@@ -9,7 +9,7 @@ using namespace b2g;
 struct b2g_i8_op {
   b2g_i8_fields f;
   int planes, device, num_sms;
-  size_t off_codes, off_scales, bytes;  // workspace layout
+  size_t off_codes, off_scales, off_partials, bytes;  // workspace: counters, codes, scales, partials
   long long ld_codes;
 };
 
@@ -32,10 +32,20 @@ bool rows16(const void* p, int64_t ld, int64_t cols, int bytes) {
   return p && aligned(p, 16) && ld >= cols && ld * bytes % 16 == 0;
 }
 
-b2g_status current_device(int* dev, int* sms) {
-  if (cudaGetDevice(dev) != cudaSuccess) return B2G_ERR_CUDA;
-  if (sms && cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess) return B2G_ERR_CUDA;
-  return B2G_OK;
+b2g_status current_device(int* dev) { return cudaGetDevice(dev) == cudaSuccess ? B2G_OK : B2G_ERR_CUDA; }
+
+// The device an op is made for.  On a machine without one (build-time sizing)
+// the op has a B200's SM count: it answers sizes and checks arguments, and
+// its enqueue returns B2G_ERR_CUDA.
+b2g_status op_device(int* dev, int* sms) {
+  const cudaError_t e = cudaGetDevice(dev);
+  if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver) {
+    *dev = -1;
+    *sms = 148;
+    return B2G_OK;
+  }
+  if (e != cudaSuccess) return B2G_ERR_CUDA;
+  return cuda_status(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev));
 }
 
 b2g_status check_cache(const b2g_kv_cache* c, int32_t act) {
@@ -115,7 +125,7 @@ b2g_status b2g_i8_create(const b2g_i8_fields* f, b2g_i8_op** out) {
   if (f->in_features > B2G_I8_MAX_K) return B2G_ERR_UNSUPPORTED;
   if (f->out_features > (1 << 24) || f->max_m > (1 << 20)) return B2G_ERR_UNSUPPORTED;
   int dev = -1, sms = 0;
-  const b2g_status st = current_device(&dev, &sms);
+  const b2g_status st = op_device(&dev, &sms);
   if (st != B2G_OK) return st;
   b2g_i8_op* op = new (std::nothrow) b2g_i8_op();
   if (!op) return B2G_ERR_OOM;
@@ -124,9 +134,10 @@ b2g_status b2g_i8_create(const b2g_i8_fields* f, b2g_i8_op** out) {
   op->device = dev;
   op->num_sms = sms;
   op->ld_codes = (long long)up(f->in_features, 16);
-  op->off_codes = 0;
-  op->off_scales = up((size_t)op->ld_codes * f->max_m, 256);
-  op->bytes = op->off_scales + up((size_t)f->max_m * 4, 256);
+  op->off_codes = up((size_t)sms * 4, 256);
+  op->off_scales = op->off_codes + up((size_t)op->ld_codes * f->max_m, 256);
+  op->off_partials = op->off_scales + up((size_t)f->max_m * 4, 256);
+  op->bytes = op->off_partials + i8_partial_bytes(f->max_m, op->planes, sms);
   *out = op;
   return B2G_OK;
 }
@@ -144,7 +155,7 @@ b2g_status b2g_i8_workspace_size(const b2g_i8_op* op, size_t* bytes) {
 
 b2g_status b2g_i8_workspace_init(const b2g_i8_op* op, void* ws, b2g_stream_t stream) {
   if (!op || !ws || !aligned(ws, 256)) return B2G_ERR_INVALID;
-  return cuda_status(cudaMemsetAsync(ws, 0, op->bytes, cu(stream)));
+  return cuda_status(cudaMemsetAsync(ws, 0, op->off_codes, cu(stream)));
 }
 
 b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* a, b2g_stream_t stream) {
@@ -165,9 +176,11 @@ b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* a, b2g_stream_
   if (resid != (a->residual != nullptr) || (resid && (!aligned(a->residual, 2) || a->ldr < N))) return B2G_ERR_INVALID;
   if (!a->workspace || !aligned(a->workspace, 256)) return B2G_ERR_INVALID;
   int dev = -1;
-  b2g_status st = current_device(&dev, nullptr);
+  b2g_status st = current_device(&dev);
   if (st != B2G_OK) return st;
   if (dev != op->device) return B2G_ERR_INVALID;
+  int* error = registered_error_word(dev);
+  if (!error) return B2G_ERR_CUDA;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   I8Params p = {};
   if (a->x) {
@@ -205,7 +218,9 @@ b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* a, b2g_stream_
   p.k = K;
   p.planes = op->planes;
   p.bf16 = op->f.dtype == B2G_DTYPE_BF16;
-  return cuda_status(launch_i8_product(p, cu(stream)));
+  return cuda_status(launch_i8_product(p, op->num_sms, reinterpret_cast<int*>(ws),
+                                       reinterpret_cast<int*>(ws + op->off_partials), error, a->x != nullptr,
+                                       cu(stream)));
 }
 
 // ---------------------------------------------------------------------------
@@ -228,7 +243,7 @@ b2g_status b2g_kv_append(const b2g_kv_append_args* a, const b2g_kv_cache* c, con
   if (a->n_freq < 0 || a->n_freq % 8 || 2 * a->n_freq > dim) return B2G_ERR_INVALID;
   if (a->n_freq && (!a->inv_freq || !aligned(a->inv_freq, 4))) return B2G_ERR_INVALID;
   int dev = -1;
-  st = current_device(&dev, nullptr);
+  st = current_device(&dev);
   if (st != B2G_OK) return st;
   KvAppendParams p = {*a, *c, *b, registered_error_word(dev)};
   if (!p.a.inv_freq) p.a.n_freq = 0;
@@ -245,7 +260,7 @@ b2g_status b2g_attn_create(const b2g_attn_fields* f, b2g_attn** out) {
   if (f->head_dim != 64 && f->head_dim != 128) return B2G_ERR_UNSUPPORTED;
   if (f->q_heads / f->kv_heads > 32 || f->q_heads > 65535) return B2G_ERR_UNSUPPORTED;
   int dev = -1, sms = 0;
-  const b2g_status st = current_device(&dev, &sms);
+  const b2g_status st = op_device(&dev, &sms);
   if (st != B2G_OK) return st;
   b2g_attn* op = new (std::nothrow) b2g_attn();
   if (!op) return B2G_ERR_OOM;
@@ -288,7 +303,7 @@ b2g_status b2g_attn_enqueue(const b2g_attn* op, const b2g_attn_args* a, const b2
   if (!aligned(a->lse, 4) || a->window < 0 || !(a->scale > 0) || a->scale > 1e30f) return B2G_ERR_INVALID;
   if (!a->workspace || !aligned(a->workspace, 256)) return B2G_ERR_INVALID;
   int dev = -1;
-  st = current_device(&dev, nullptr);
+  st = current_device(&dev);
   if (st != B2G_OK) return st;
   if (dev != op->device) return B2G_ERR_INVALID;
   AttnParams p = {};
