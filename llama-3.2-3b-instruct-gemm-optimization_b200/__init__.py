@@ -14,6 +14,7 @@ IPluginV3 creator (tensorrt_custom_tactic_kernel_b07f17a4.plan.md:57-58) and
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -175,20 +176,19 @@ SIGNATURES = {
     "b2g_stack_workspace_size": ([_P, _I32, ctypes.POINTER(_SZ)], ctypes.c_int),
     "b2g_stack_workspace_init": ([_P, _P, _P], ctypes.c_int),
     "b2g_stack_enqueue": ([_P, _I32, _P, _P, _P, _P], ctypes.c_int),
-    "b2g_i8_quantize_rows": ([ctypes.POINTER(I8RowsArgs), _P], ctypes.c_int),
+    "b2g_i8_quantize_rows": ([_P, _P], ctypes.c_int),
     "b2g_i8_quantize_weights": ([_P, _I32, _I32, _I32, _I32, _P, _I64, _P, _P], ctypes.c_int),
     "b2g_i8_create": ([ctypes.POINTER(I8Fields), ctypes.POINTER(_P)], ctypes.c_int),
     "b2g_i8_destroy": ([_P], ctypes.c_int),
     "b2g_i8_workspace_size": ([_P, ctypes.POINTER(_SZ)], ctypes.c_int),
     "b2g_i8_workspace_init": ([_P, _P, _P], ctypes.c_int),
-    "b2g_i8_enqueue": ([_P, ctypes.POINTER(I8Args), _P], ctypes.c_int),
-    "b2g_kv_append": ([ctypes.POINTER(KvAppendArgs), ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), _P],
-                      ctypes.c_int),
+    "b2g_i8_enqueue": ([_P, _P, _P], ctypes.c_int),
+    "b2g_kv_append": ([_P, _P, _P, _P], ctypes.c_int),
     "b2g_attn_create": ([ctypes.POINTER(AttnFields), ctypes.POINTER(_P)], ctypes.c_int),
     "b2g_attn_destroy": ([_P], ctypes.c_int),
     "b2g_attn_workspace_size": ([_P, ctypes.POINTER(_SZ)], ctypes.c_int),
     "b2g_attn_workspace_init": ([_P, _P, _P], ctypes.c_int),
-    "b2g_attn_enqueue": ([_P, ctypes.POINTER(AttnArgs), ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), _P],
+    "b2g_attn_enqueue": ([_P, _P, _P, _P, _P],
                          ctypes.c_int),
 }
 
@@ -498,63 +498,103 @@ def tp_gather(comm, buf: int, push_op, h, stream=None):
 
 # ---------------------------------------------------------------------------
 # 8-bit integer product, paged cache, attention
+#
+# A decode step's calls take a few microseconds on the device, so what one
+# costs in Python is kept small: argument structures are packed into bytes
+# (a fifth of a ctypes.Structure's time), a tensor's shape, type and strides
+# are read once.
 # ---------------------------------------------------------------------------
+def _packer(fields):
+    """Packs a ctypes.Structure's fields into bytes of its layout (pointers as integers)."""
+    code = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_void_p: "P", ctypes.c_float: "f"}
+    s = struct.Struct("@" + "".join(code[t] for _, t in fields._fields_) + "0q")
+    assert s.size == ctypes.sizeof(fields)
+    return s.pack
+
+
+_pack_rows, _pack_i8, _pack_cache, _pack_batch, _pack_append, _pack_attn = map(
+    _packer, (I8RowsArgs, I8Args, KvCache, KvBatch, KvAppendArgs, AttnArgs))
+_ACT_CODE, _ACT_TYPE, _CACHE_CODE = {}, {}, {}
+
+
+def _types():
+    """torch's types by B2G_DTYPE_* code, and back (torch is imported on first use)."""
+    if not _ACT_CODE:
+        import torch
+        _ACT_TYPE.update({0: torch.float16, 2: torch.bfloat16})
+        _CACHE_CODE.update({torch.float16: 0, torch.float8_e4m3fn: 1, torch.bfloat16: 2})
+        _ACT_CODE.update({t: c for c, t in _ACT_TYPE.items()})
+    return _ACT_TYPE
+
+
 def _act_code(t):
-    """B2G_DTYPE_* of 16-bit activations."""
+    _types()
+    code = _ACT_CODE.get(t.dtype)
+    if code is None:
+        raise ValueError(f"expected float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _launch_stream(stream, device, tensors):
+    """The raw stream to launch on, once every tensor is on the current device."""
     import torch
-    if t.dtype == torch.float16:
-        return 0
-    if t.dtype == torch.bfloat16:
-        return 2
-    raise ValueError(f"expected float16 or bfloat16, got {t.dtype}")
-
-
-def _act_type(code):
-    import torch
-    return {0: torch.float16, 2: torch.bfloat16}[code]
-
-
-def _on(device, *tensors):
-    """The current device holds every tensor (the library launches there)."""
-    import torch
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
+    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
         raise ValueError(f"tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
     for t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f"tensors on {device} and {t.device}")
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    if stream.device != device:
+        raise ValueError(f"tensors on {device}, a stream of {stream.device}")
+    return stream.cuda_stream
 
 
-def _matrix(t, dtype, rows, cols, what):
-    if t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: expected [{rows}, {cols}] {dtype} with contiguous rows, got {tuple(t.shape)} "
-                         f"{t.dtype} strides {t.stride()}")
+def _made(stream, make):
+    """A buffer that a call makes for its work on `stream`: allocated under
+    that stream, so that the allocator does not hand it on before that work is
+    done."""
+    if stream is None:
+        return make()
+    import torch
+    with torch.cuda.stream(stream):
+        return make()
 
 
-def _ld(t, align):
-    """Row stride in elements; a single row may carry any, so it gets an aligned one."""
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // align) * align
+def _matrix(t, dtype, shape, align, what):
+    """The row stride of a matrix with contiguous rows (a single row may carry
+    any stride, so it gets an aligned one)."""
+    if t.dtype is dtype and t.shape == shape:
+        rows, cols = t.stride()
+        if cols == 1 or shape[1] == 1:
+            return rows if shape[0] > 1 else -(-shape[1] // align) * align
+    raise ValueError(f"{what}: expected {list(shape)} {dtype} with contiguous rows, got {tuple(t.shape)} {t.dtype} "
+                     f"strides {t.stride()}")
 
 
 def _vector(t, dtype, n, what):
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
+    if t.dtype is not dtype or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
         raise ValueError(f"{what}: expected {n} contiguous {dtype}, got {tuple(t.shape)} {t.dtype}")
 
 
-class _Made:
-    """Buffers that a call makes for itself on `stream`: made under that
-    stream, so the allocator does not hand them on before its work is done."""
+def _heads(t, shape, dtype, what):
+    """(address, row stride, head stride) of [rows, heads, dim]."""
+    if t.dtype is dtype and t.shape == shape:
+        row, head, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), row, head
+    raise ValueError(f"{what}: expected {list(shape)} {dtype} with a contiguous last axis, got {tuple(t.shape)} "
+                     f"{t.dtype} strides {t.stride()}")
 
-    def __init__(self, stream):
-        import torch
-        self.ctx = None if stream is None else torch.cuda.stream(stream)
 
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
+def _workspace(ws, need):
+    if ws.nbytes < need or not ws.is_contiguous():
+        raise ValueError(f"the workspace needs {need} contiguous bytes")
+    return ws.data_ptr()
 
-    def __exit__(self, *a):
-        if self.ctx is not None:
-            self.ctx.__exit__(*a)
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _codes(rows, cols, device):
@@ -570,21 +610,19 @@ def quantize_i8_rows(x, gamma=None, rms_eps=None, codes=None, scales=None, strea
     """
     import torch
     m, k = x.shape
-    _on(x.device, x, gamma, codes, scales)
-    _matrix(x, x.dtype, m, k, "x")
+    raw = _launch_stream(stream, x.device, (gamma, codes, scales))
+    ldx = _matrix(x, x.dtype, (m, k), 8, "x")
     if gamma is not None:
         _vector(gamma, x.dtype, k, "gamma")
-    with _Made(stream):
-        if codes is None:
-            codes = _codes(m, k, x.device)
-        if scales is None:
-            scales = torch.empty(m, dtype=torch.float32, device=x.device)
-    _matrix(codes, torch.int8, m, k, "codes")
+    if codes is None:
+        codes = _made(stream, lambda: _codes(m, k, x.device))
+    if scales is None:
+        scales = _made(stream, lambda: torch.empty(m, dtype=torch.float32, device=x.device))
+    ldc = _matrix(codes, torch.int8, (m, k), 16, "codes")
     _vector(scales, torch.float32, m, "scales")
-    a = I8RowsArgs(m, k, _act_code(x), rms_eps is not None, x.data_ptr(), _ld(x, 8),
-                   None if gamma is None else gamma.data_ptr(), rms_eps or 0.0, codes.data_ptr(), _ld(codes, 16),
-                   scales.data_ptr())
-    check(lib().b2g_i8_quantize_rows(ctypes.byref(a), _stream(stream)), "b2g_i8_quantize_rows")
+    a = _pack_rows(m, k, _act_code(x), rms_eps is not None, x.data_ptr(), ldx, _address(gamma), rms_eps or 0.0,
+                   codes.data_ptr(), ldc, scales.data_ptr())
+    check(lib().b2g_i8_quantize_rows(a, raw), "b2g_i8_quantize_rows")
     return codes, scales
 
 
@@ -593,14 +631,13 @@ def quantize_i8_weights(w16, layout="KN", stream=None):
     import torch
     lay = _code(LAYOUT, layout)
     K, N = (w16.shape if lay == 0 else w16.shape[::-1])
-    _on(w16.device, w16)
+    raw = _launch_stream(stream, w16.device, ())
     if not w16.is_contiguous():
         raise ValueError("w16 must be contiguous")
-    with _Made(stream):
-        codes = _codes(N, K, w16.device)
-        scales = torch.empty(N, dtype=torch.float32, device=w16.device)
-    check(lib().b2g_i8_quantize_weights(_ptr(w16), K, N, lay, _act_code(w16), _ptr(codes), _ld(codes, 16),
-                                        _ptr(scales), _stream(stream)), "b2g_i8_quantize_weights")
+    codes = _made(stream, lambda: _codes(N, K, w16.device))
+    scales = _made(stream, lambda: torch.empty(N, dtype=torch.float32, device=w16.device))
+    check(lib().b2g_i8_quantize_weights(_ptr(w16), K, N, lay, _act_code(w16), _ptr(codes), -(-K // 16) * 16,
+                                        _ptr(scales), raw), "b2g_i8_quantize_weights")
     return codes, scales
 
 
@@ -616,11 +653,13 @@ class I8Op:
         self.K, self.N, self.max_m, self.fuse = in_features, out_features, max_m, fuse
         self.dtype = _code(DTYPE, dtype)
         self.planes = 2 if fuse & FUSE_GATE_UP_SILU else 1
-        h = ctypes.c_void_p()
+        h, n = ctypes.c_void_p(), ctypes.c_size_t()
         f = I8Fields(in_features, out_features, max_m, self.dtype, fuse)
         check(lib().b2g_i8_create(ctypes.byref(f), ctypes.byref(h)), "b2g_i8_create")
         self.h = h
-        self._type = _act_type(self.dtype)
+        check(lib().b2g_i8_workspace_size(self.h, ctypes.byref(n)), "b2g_i8_workspace_size")
+        self._ws_bytes = n.value
+        self._type = _types()[self.dtype]
 
     def __del__(self):
         if getattr(self, "h", None) and _lib is not None:
@@ -628,59 +667,56 @@ class I8Op:
             self.h = None
 
     def workspace_bytes(self) -> int:
-        n = ctypes.c_size_t()
-        check(lib().b2g_i8_workspace_size(self.h, ctypes.byref(n)), "b2g_i8_workspace_size")
-        return n.value
+        return self._ws_bytes
 
     def workspace(self, device="cuda", stream=None):
-        """A zeroed workspace.  Calls that can overlap (other streams, graphs
-        replayed at the same time) need one each."""
+        """A zeroed workspace.  Calls that can overlap (other
+        streams, graphs replayed at the same time) need one each."""
         import torch
-        with _Made(stream):
-            ws = torch.empty(self.workspace_bytes(), dtype=torch.uint8, device=device)
+        ws = _made(stream, lambda: torch.empty(self._ws_bytes, dtype=torch.uint8, device=device))
         check(lib().b2g_i8_workspace_init(self.h, _ptr(ws), _stream(stream)), "b2g_i8_workspace_init")
         return ws
-
-    def _enqueue(self, m, x, gamma, rms_eps, codes, scales, wq, sw, residual, y, workspace, stream):
-        import torch
-        first = x if codes is None else codes
-        _on(first.device, gamma, scales, wq, sw, residual, y, workspace)
-        _matrix(wq, torch.int8, self.planes * self.N, self.K, "wq")
-        _vector(sw, torch.float32, self.planes * self.N, "sw")
-        if residual is not None:
-            _matrix(residual, self._type, m, self.N, "residual")
-        if y is None:
-            with _Made(stream):
-                y = torch.empty((m, self.N), dtype=self._type, device=first.device)
-        else:
-            _matrix(y, self._type, m, self.N, "y")
-        if workspace is None:
-            workspace = self.workspace(first.device, stream)
-        elif workspace.numel() * workspace.element_size() < self.workspace_bytes() or not workspace.is_contiguous():
-            raise ValueError(f"the workspace needs {self.workspace_bytes()} contiguous bytes")
-        a = I8Args(m, None if x is None else x.data_ptr(), 0 if x is None else _ld(x, 8),
-                   None if gamma is None else gamma.data_ptr(), rms_eps,
-                   None if codes is None else codes.data_ptr(), 0 if codes is None else _ld(codes, 16),
-                   None if scales is None else scales.data_ptr(), wq.data_ptr(), _ld(wq, 16), sw.data_ptr(),
-                   None if residual is None else residual.data_ptr(), 0 if residual is None else _ld(residual, 1),
-                   y.data_ptr(), _ld(y, 1), workspace.data_ptr())
-        check(lib().b2g_i8_enqueue(self.h, ctypes.byref(a), _stream(stream)), "b2g_i8_enqueue")
-        return y
 
     def enqueue(self, x, wq, sw, y=None, workspace=None, residual=None, gamma=None, rms_eps: float = 1e-5,
                 stream=None):
         """y of 16-bit rows x [m, K], quantised (and normalised) on the way."""
-        _matrix(x, self._type, x.shape[0], self.K, "x")
+        m = x.shape[0]
+        ldx = _matrix(x, self._type, (m, self.K), 8, "x")
         if gamma is not None:
             _vector(gamma, self._type, self.K, "gamma")
-        return self._enqueue(x.shape[0], x, gamma, rms_eps, None, None, wq, sw, residual, y, workspace, stream)
+        raw = _launch_stream(stream, x.device, (wq, sw, y, workspace, residual, gamma))
+        return self._enqueue(m, x.device, (x.data_ptr(), ldx, _address(gamma), rms_eps, 0, 0, 0), wq, sw, y,
+                             workspace, residual, stream, raw)
 
     def enqueue_codes(self, xq, sx, wq, sw, y=None, workspace=None, residual=None, stream=None):
         """y of rows that quantize_i8_rows has quantised (one quantisation, several products)."""
         import torch
-        _matrix(xq, torch.int8, xq.shape[0], self.K, "xq")
-        _vector(sx, torch.float32, xq.shape[0], "sx")
-        return self._enqueue(xq.shape[0], None, None, 0.0, xq, sx, wq, sw, residual, y, workspace, stream)
+        m = xq.shape[0]
+        ldx = _matrix(xq, torch.int8, (m, self.K), 16, "xq")
+        _vector(sx, torch.float32, m, "sx")
+        raw = _launch_stream(stream, xq.device, (sx, wq, sw, y, workspace, residual))
+        return self._enqueue(m, xq.device, (0, 0, 0, 0.0, xq.data_ptr(), ldx, sx.data_ptr()), wq, sw, y, workspace,
+                             residual, stream, raw)
+
+    def _enqueue(self, m, device, x_args, wq, sw, y, workspace, residual, stream, raw):
+        import torch
+        rows = self.planes * self.N
+        ldw = _matrix(wq, torch.int8, (rows, self.K), 16, "wq")
+        _vector(sw, torch.float32, rows, "sw")
+        ldr = 0 if residual is None else _matrix(residual, self._type, (m, self.N), 1, "residual")
+        if y is None:
+            y = _made(stream, lambda: torch.empty((m, self.N), dtype=self._type, device=device))
+            ldy = self.N
+        else:
+            ldy = _matrix(y, self._type, (m, self.N), 1, "y")
+        if workspace is None:
+            workspace = self.workspace(device, stream)
+        a = _pack_i8(m, *x_args, wq.data_ptr(), ldw, sw.data_ptr(), _address(residual), ldr, y.data_ptr(), ldy,
+                     _workspace(workspace, self._ws_bytes))
+        status = lib().b2g_i8_enqueue(self.h, a, raw)
+        if status:
+            check(status, "b2g_i8_enqueue")
+        return y
 
 
 class PagedCache:
@@ -693,7 +729,8 @@ class PagedCache:
         import torch
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("k and v: two 4-d tensors of one shape, type and strides, the last axis contiguous")
-        code = {torch.float16: 0, torch.bfloat16: 2, torch.float8_e4m3fn: 1}.get(k.dtype)
+        _types()
+        code = _CACHE_CODE.get(k.dtype)
         if code is None or layout not in ("NHD", "HND"):
             raise ValueError(f"cache type {k.dtype}, layout {layout}")
         tok, head = (1, 2) if layout == "NHD" else (2, 1)
@@ -704,30 +741,23 @@ class PagedCache:
             raise ValueError("the cache's tensors are on different devices")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.page_size, self.kv_heads, self.head_dim, self.dtype = k.shape[tok], k.shape[head], k.shape[3], code
-        self.c = KvCache(k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
-                         None if v_scale is None else v_scale.data_ptr(), k.stride(0), k.stride(tok),
-                         k.stride(head), k.shape[0], self.page_size, self.kv_heads, self.head_dim, code)
+        # The tensors are held above, so their addresses stay theirs.
+        self.packed = _pack_cache(k.data_ptr(), v.data_ptr(), _address(k_scale), _address(v_scale), k.stride(0),
+                                  k.stride(tok), k.stride(head), k.shape[0], self.page_size, self.kv_heads,
+                                  self.head_dim, code)
 
 
-def _kv_batch(device, rows, q_start, seq_lens, page_table, max_q):
+def _batch(rows, q_start, seq_lens, page_table, max_q):
     import torch
     batch = seq_lens.shape[0]
-    _on(device, q_start, seq_lens, page_table)
     _vector(q_start, torch.int32, batch + 1, "q_start")
     _vector(seq_lens, torch.int32, batch, "seq_lens")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or \
-            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError(f"page_table: expected [{batch}, pages] int32 with contiguous rows")
-    return KvBatch(batch, rows, max_q or rows, page_table.shape[1], _ld(page_table, 1), q_start.data_ptr(),
-                   seq_lens.data_ptr(), page_table.data_ptr())
-
-
-def _heads(t, rows, heads, dim, dtype, what):
-    if t.dtype != dtype or t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != dim or \
-            t.stride(2) != 1:
-        raise ValueError(f"{what}: expected [{rows}, {heads}, {dim}] {dtype} with a contiguous last axis, got "
-                         f"{tuple(t.shape)} {t.dtype} strides {t.stride()}")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    if page_table.dim() != 2:
+        raise ValueError("page_table: expected [batch, pages]")
+    pages = page_table.shape[1]
+    ld = _matrix(page_table, torch.int32, (batch, pages), 1, "page_table")
+    return _pack_batch(batch, rows, rows if max_q is None else max_q, pages, ld, q_start.data_ptr(),
+                       seq_lens.data_ptr(), page_table.data_ptr())
 
 
 def kv_append(k, v, cache, q_start, seq_lens, page_table, q=None, q_out=None, inv_freq=None,
@@ -740,23 +770,24 @@ def kv_append(k, v, cache, q_start, seq_lens, page_table, q=None, q_out=None, in
     of a head by pos * inv_freq (None: no rotation).
     """
     import torch
-    rows, dim = k.shape[0], cache.head_dim
-    _on(k.device, v, cache.k, q, q_out, inv_freq)
-    b = _kv_batch(k.device, rows, q_start, seq_lens, page_table, 0)
-    kk = _heads(k, rows, cache.kv_heads, dim, k.dtype, "k")
-    vv = _heads(v, rows, cache.kv_heads, dim, k.dtype, "v")
-    qq = qo = (None, 0, 0)
+    rows, dim, t = k.shape[0], cache.head_dim, k.dtype
+    raw = _launch_stream(stream, k.device, (v, cache.k, q_start, seq_lens, page_table, q, q_out, inv_freq))
+    shape = (rows, cache.kv_heads, dim)
+    heads, qq, qo, n_freq = 0, (0, 0, 0), (0, 0, 0), 0
     if q is not None:
-        qq = _heads(q, rows, q.shape[1], dim, k.dtype, "q")
-        qo = qq if q_out is None else _heads(q_out, rows, q.shape[1], dim, k.dtype, "q_out")
+        heads = q.shape[1]
+        qq = _heads(q, (rows, heads, dim), t, "q")
+        qo = qq if q_out is None else _heads(q_out, (rows, heads, dim), t, "q_out")
     elif q_out is not None:
         raise ValueError("q_out without q")
     if inv_freq is not None:
-        _vector(inv_freq, torch.float32, inv_freq.shape[0], "inv_freq")
-    a = KvAppendArgs(_act_code(k), 0 if q is None else q.shape[1], 0 if inv_freq is None else inv_freq.shape[0],
-                     1 if interleaved else 0, None if inv_freq is None else inv_freq.data_ptr(), *kk, *vv, *qq, *qo)
-    check(lib().b2g_kv_append(ctypes.byref(a), ctypes.byref(cache.c), ctypes.byref(b), _stream(stream)),
-          "b2g_kv_append")
+        n_freq = inv_freq.shape[0]
+        _vector(inv_freq, torch.float32, n_freq, "inv_freq")
+    a = _pack_append(_act_code(k), heads, n_freq, interleaved, _address(inv_freq), *_heads(k, shape, t, "k"),
+                     *_heads(v, shape, t, "v"), *qq, *qo)
+    status = lib().b2g_kv_append(a, cache.packed, _batch(rows, q_start, seq_lens, page_table, 1), raw)
+    if status:
+        check(status, "b2g_kv_append")
     return q if q_out is None else q_out
 
 
@@ -768,11 +799,13 @@ class AttnOp:
         self.q_heads, self.kv_heads, self.head_dim, self.max_batch = q_heads, kv_heads, head_dim, max_batch
         self.dtype = _code(DTYPE, dtype)
         self.cache_dtype = self.dtype if cache_dtype is None else _code(DTYPE, cache_dtype)
-        h = ctypes.c_void_p()
+        h, n = ctypes.c_void_p(), ctypes.c_size_t()
         f = AttnFields(q_heads, kv_heads, head_dim, max_batch, self.dtype, self.cache_dtype)
         check(lib().b2g_attn_create(ctypes.byref(f), ctypes.byref(h)), "b2g_attn_create")
         self.h = h
-        self._type = _act_type(self.dtype)
+        check(lib().b2g_attn_workspace_size(self.h, ctypes.byref(n)), "b2g_attn_workspace_size")
+        self._ws_bytes = n.value
+        self._type = _types()[self.dtype]
 
     def __del__(self):
         if getattr(self, "h", None) and _lib is not None:
@@ -780,16 +813,13 @@ class AttnOp:
             self.h = None
 
     def workspace_bytes(self) -> int:
-        n = ctypes.c_size_t()
-        check(lib().b2g_attn_workspace_size(self.h, ctypes.byref(n)), "b2g_attn_workspace_size")
-        return n.value
+        return self._ws_bytes
 
     def workspace(self, device="cuda", stream=None):
-        """A zeroed workspace.  Calls that can overlap (other streams, graphs
-        replayed at the same time) need one each."""
+        """A zeroed workspace.  Calls that can overlap (other
+        streams, graphs replayed at the same time) need one each."""
         import torch
-        with _Made(stream):
-            ws = torch.empty(self.workspace_bytes(), dtype=torch.uint8, device=device)
+        ws = _made(stream, lambda: torch.empty(self._ws_bytes, dtype=torch.uint8, device=device))
         check(lib().b2g_attn_workspace_init(self.h, _ptr(ws), _stream(stream)), "b2g_attn_workspace_init")
         return ws
 
@@ -802,23 +832,23 @@ class AttnOp:
         the last `window` positions, its own among them (0: all).
         """
         import torch
-        rows = q.shape[0]
-        _on(q.device, cache.k, out, lse, workspace)
-        b = _kv_batch(q.device, rows, q_start, seq_lens, page_table, max_q)
-        qq = _heads(q, rows, self.q_heads, self.head_dim, self._type, "q")
+        rows, device = q.shape[0], q.device
+        raw = _launch_stream(stream, device, (cache.k, q_start, seq_lens, page_table, out, lse, workspace))
+        shape = (rows, self.q_heads, self.head_dim)
+        qq = _heads(q, shape, self._type, "q")
         if out is None:
-            with _Made(stream):
-                out = torch.empty((rows, self.q_heads, self.head_dim), dtype=self._type, device=q.device)
-        oo = _heads(out, rows, self.q_heads, self.head_dim, self._type, "out")
-        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (rows, self.q_heads) or
-                                not lse.is_contiguous()):
+            out = _made(stream, lambda: torch.empty(shape, dtype=self._type, device=device))
+            oo = (out.data_ptr(), self.q_heads * self.head_dim, self.head_dim)
+        else:
+            oo = _heads(out, shape, self._type, "out")
+        if lse is not None and (lse.dtype is not torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
             raise ValueError(f"lse: expected [{rows}, {self.q_heads}] contiguous float32")
         if workspace is None:
-            workspace = self.workspace(q.device, stream)
-        elif workspace.numel() * workspace.element_size() < self.workspace_bytes() or not workspace.is_contiguous():
-            raise ValueError(f"the workspace needs {self.workspace_bytes()} contiguous bytes")
-        a = AttnArgs(*qq, *oo, None if lse is None else lse.data_ptr(),
-                     self.head_dim ** -0.5 if scale is None else scale, window, workspace.data_ptr())
-        check(lib().b2g_attn_enqueue(self.h, ctypes.byref(a), ctypes.byref(cache.c), ctypes.byref(b),
-                                     _stream(stream)), "b2g_attn_enqueue")
+            workspace = self.workspace(device, stream)
+        a = _pack_attn(*qq, *oo, _address(lse), self.head_dim ** -0.5 if scale is None else scale, window,
+                       _workspace(workspace, self._ws_bytes))
+        status = lib().b2g_attn_enqueue(self.h, a, cache.packed, _batch(rows, q_start, seq_lens, page_table, max_q),
+                                        raw)
+        if status:
+            check(status, "b2g_attn_enqueue")
         return out

@@ -1,59 +1,152 @@
 // i8.cu -- matrix product in 8-bit integers with a scale for each row of x
 // and each output channel, and the quantisers that make its operands.
+#include <atomic>
+
+#include <algorithm>
+
 #include "serve.cuh"
 #include "tc.cuh"
 
 namespace b2g {
 namespace {
 
-// v / s rounded to the nearest integer, ties to even (a row that is not
-// finite has s = NaN and zero codes).
-__device__ __forceinline__ int code_of(float v, float s) { return s == s ? __float2int_rn(v / s) : 0; }
+// v / s rounded to the nearest integer, ties to even, as v * (1 / s): a
+// quotient within 2^-23 of a tie may go the other way.  Adding 1.5 * 2^23
+// leaves the integer in the low bits, in one fused multiply-add a value.
+__device__ __forceinline__ uint32_t code_of(float v, float inv) {
+  return __float_as_uint(__fmaf_rn(v, inv, 12582912.0f)) & 0xff;
+}
 __device__ __forceinline__ float scale_of(float amax) {
   return amax <= 3.4028235e38f ? fmaxf(amax, 1e-12f) / 127.0f : __uint_as_float(0x7fffffffu);
 }
-// Maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) { return a > b || a != a ? a : b; }
+// Maximum of absolute values that keeps a NaN: as integers the patterns of
+// |v| are in order, infinity above the finite ones and NaNs on top.
+__device__ __forceinline__ float max_abs(float a, float v) {
+  return __uint_as_float(max(__float_as_uint(a), __float_as_uint(v) & 0x7fffffffu));
+}
 
+// Elements 8c .. 8c + 7 of a row of k (zeros behind its end).
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const I8RowsParams p) {
-  pdl_launch_dependents();
-  __shared__ float red[8];
-  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ void load8(const T* row, int c, int k, float (&f)[8]) {
+  if (8 * c + 8 <= k) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + 8 * c);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = Act<T>::unpack(w[i]);
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 8 * c + i < k ? Act<T>::to_float(row[8 * c + i]) : 0.f;
+  }
+}
+
+// One block a row.  A thread keeps up to 32 elements (four 16-byte loads) in
+// registers, so a row of up to 32 x threads elements is read once; a longer
+// one is read again for each pass.
+template <typename T, bool RMS>
+__global__ void __launch_bounds__(512) quantize_rows_kernel(const I8RowsParams p) {
+  constexpr int NC = 4;
+  __shared__ float red[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* gamma = static_cast<const T*>(p.gamma);
+  const int chunks = (p.k + 7) / 8, per_pass = NC * blockDim.x;
+  const bool resident = chunks <= per_pass;
+  pdl_wait();
+  pdl_launch_dependents();  // behind the wait: the launch after this one may read weights at once
+  float v[NC][8];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = base + i * blockDim.x + threadIdx.x;
+      if (c < chunks) {
+        load8(x, c, p.k, v[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+      }
+    }
+  };
   float r = 1.0f;
-  if (p.rmsnorm) {
+  auto normalise = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = base + i * blockDim.x + threadIdx.x;
+      if (c >= chunks) continue;
+      float g[8];
+      if (gamma) load8(gamma, c, p.k, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = gamma ? v[i][e] * r * g[e] : v[i][e] * r;
+    }
+  };
+  load(0);
+  if constexpr (RMS) {
     float ss = 0.f;
-    for (int i = threadIdx.x; i < p.k; i += 256) {
-      const float v = Act<T>::to_float(x[i]);
-      ss += v * v;
+    for (int base = 0; base < chunks; base += per_pass) {
+      if (base) load(base);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
     }
     for (int off = 16; off; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    if (lane == 0) red[warp] = ss;
+    if (lane == 0) red[0][warp] = ss;
     __syncthreads();
-    ss = 0.f;
-    for (int w = 0; w < 8; ++w) ss += red[w];
+    ss = lane < warps ? red[0][lane] : 0.f;
+    for (int off = 16; off; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     r = rsqrtf(ss / (float)p.k + p.eps);
-    __syncthreads();
+    if (!resident) load(0);
+    normalise(0);
   }
   float a = 0.f;
-  for (int i = threadIdx.x; i < p.k; i += 256) {
-    float v = Act<T>::to_float(x[i]) * r;
-    if (gamma) v *= Act<T>::to_float(gamma[i]);
-    a = max_nan(a, fabsf(v));
+  for (int base = 0; base < chunks; base += per_pass) {
+    if (base) {
+      load(base);
+      if constexpr (RMS) normalise(base);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = max_abs(a, v[i][e]);
   }
-  for (int off = 16; off; off >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, off));
-  if (lane == 0) red[warp] = a;
+  for (int off = 16; off; off >>= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, off));
+  if (lane == 0) red[1][warp] = a;
   __syncthreads();
-  for (int w = 0; w < 8; ++w) a = max_nan(a, red[w]);
+  a = lane < warps ? red[1][lane] : 0.f;
+  for (int off = 16; off; off >>= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, off));
   const float s = scale_of(a);
-  for (int i = threadIdx.x; i < p.k; i += 256) {
-    float v = Act<T>::to_float(x[i]) * r;
-    if (gamma) v *= Act<T>::to_float(gamma[i]);
-    p.codes[row * p.ldc + i] = (int8_t)code_of(v, s);
+  const bool finite = s == s;
+  const float inv = 1.0f / s;
+  int8_t* codes = p.codes + row * p.ldc;
+  for (int base = 0; base < chunks; base += per_pass) {
+    if (!resident) {
+      load(base);
+      if constexpr (RMS) normalise(base);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = base + i * blockDim.x + threadIdx.x;
+      if (c >= chunks) continue;
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e / 4] |= (finite ? code_of(v[i][e], inv) : 0) << (8 * (e % 4));
+      if (8 * c + 8 <= p.k) {
+        *reinterpret_cast<uint2*>(codes + 8 * c) = make_uint2(w[0], w[1]);
+      } else {
+        for (int e = 0; 8 * c + e < p.k; ++e) codes[8 * c + e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
+      }
+    }
   }
   if (threadIdx.x == 0) p.scales[row] = s;
+}
+
+// The code of a weight; a channel that is not finite (inv 0) has zero codes.
+__device__ __forceinline__ int8_t channel_code(float v, float inv) {
+  return inv > 0.f ? (int8_t)code_of(v, inv) : (int8_t)0;
 }
 
 // One-off: 32 output channels a block, both passes over K.
@@ -62,36 +155,36 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
                                                                 int8_t* __restrict__ codes, long long ldc,
                                                                 float* __restrict__ scales) {
   __shared__ float tile[32][33];
-  __shared__ float sc[32];
+  __shared__ float inv[32];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n0 = blockIdx.x * 32;
   float a = 0.f;
   // KN: lanes over channels; NK: lanes over k, a warp per channel.
   if (layout == B2G_LAYOUT_KN) {
     if (n0 + tx < N)
-      for (int k = ty; k < K; k += 32) a = max_nan(a, fabsf(Act<T>::to_float(w[(long long)k * N + n0 + tx])));
+      for (int k = ty; k < K; k += 32) a = max_abs(a, Act<T>::to_float(w[(long long)k * N + n0 + tx]));
     tile[ty][tx] = a;
   } else {
     if (n0 + ty < N)
-      for (int k = tx; k < K; k += 32) a = max_nan(a, fabsf(Act<T>::to_float(w[(long long)(n0 + ty) * K + k])));
+      for (int k = tx; k < K; k += 32) a = max_abs(a, Act<T>::to_float(w[(long long)(n0 + ty) * K + k]));
     tile[tx][ty] = a;
   }
   __syncthreads();
   if (ty == 0) {
-    for (int i = 0; i < 32; ++i) a = max_nan(a, tile[i][tx]);
-    sc[tx] = scale_of(a);
-    if (n0 + tx < N) scales[n0 + tx] = sc[tx];
+    for (int i = 0; i < 32; ++i) a = max_abs(a, tile[i][tx]);
+    const float s = scale_of(a);
+    inv[tx] = s == s ? 1.0f / s : 0.f;
+    if (n0 + tx < N) scales[n0 + tx] = s;
   }
   __syncthreads();
   for (int k0 = 0; k0 < K; k0 += 32) {
     if (layout == B2G_LAYOUT_KN) {
       if (k0 + ty < K && n0 + tx < N) tile[ty][tx] = Act<T>::to_float(w[(long long)(k0 + ty) * N + n0 + tx]);
       __syncthreads();
-      if (n0 + ty < N && k0 + tx < K) codes[(n0 + ty) * ldc + k0 + tx] = (int8_t)code_of(tile[tx][ty], sc[ty]);
+      if (n0 + ty < N && k0 + tx < K) codes[(n0 + ty) * ldc + k0 + tx] = channel_code(tile[tx][ty], inv[ty]);
       __syncthreads();
     } else if (n0 + ty < N && k0 + tx < K) {
-      codes[(n0 + ty) * ldc + k0 + tx] =
-          (int8_t)code_of(Act<T>::to_float(w[(long long)(n0 + ty) * K + k0 + tx]), sc[ty]);
+      codes[(n0 + ty) * ldc + k0 + tx] = channel_code(Act<T>::to_float(w[(long long)(n0 + ty) * K + k0 + tx]), inv[ty]);
     }
   }
 }
@@ -107,9 +200,9 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
 // matrices), warp 1 issues tcgen05.mma.kind::i8 into one of two accumulators
 // in tensor memory, warps 2..5 drain the other one.  Work is cut as whole
 // tiles where they fill the SMs, else as equal ranges of k blocks ("units"):
-// a range's tiles at its two ends are shared with other CTAs, which leave
-// their int32 sums in the workspace; the last to arrive adds them (integer
-// sums: the order does not matter) and finishes the tile.
+// a range's tiles at its two ends are shared with other CTAs, which all add
+// their int32 sums into the workspace (integers: the order does not matter);
+// the last to arrive finishes the tile and leaves zeros behind.
 // ---------------------------------------------------------------------------
 constexpr int kI8Threads = 192;
 constexpr int kI8MaxStages = 12;
@@ -121,11 +214,12 @@ struct I8Tc {
   CUtensorMap mw, mx;
   I8Params p;
   int bn, stages, kb, tok_tiles, tiles, whole;
-  int tmem_cols;
+  int cluster;          // CTAs a tile (1: none)
+  int tmem_cols, after_quantiser;
   long long units;
   long long slot_ints;  // int32 words of one partial
   int* counters;        // [grid], zero between launches
-  int* partials;        // [grid][2][slot_ints]
+  int* partials;        // [grid][slot_ints] sums of the split tile whose first k block a CTA has; zero between launches
   int* error;
 };
 
@@ -135,12 +229,23 @@ struct I8Seg {
   int tile, k0, k1;
   __device__ __forceinline__ void begin(const I8Tc& t) {
     const int c = blockIdx.x, g = gridDim.x;
+    if (t.cluster > 1) {
+      u = c;
+      end = c + 1;
+      return;
+    }
     u = t.whole ? c : c * t.units / g;
     end = t.whole ? t.tiles : (c + 1) * t.units / g;
   }
   __device__ __forceinline__ bool next(const I8Tc& t) {
     if (u >= end) return false;
-    if (t.whole) {
+    if (t.cluster > 1) {
+      const int rank = (int)u % t.cluster;
+      tile = (int)u / t.cluster;
+      k0 = rank * t.kb / t.cluster;
+      k1 = (rank + 1) * t.kb / t.cluster;
+      ++u;
+    } else if (t.whole) {
       tile = (int)u;
       k0 = 0;
       k1 = t.kb;
@@ -159,12 +264,21 @@ __device__ __forceinline__ int i8_owner(const I8Tc& t, long long u) {
   return (int)(((u + 1) * gridDim.x - 1) / t.units);
 }
 
+// The scaled sum, or SiLU(gate) * up.
+template <int PLANES>
+__device__ __forceinline__ float i8_value(int acc, int acc_up, const float (&sw)[PLANES], float sx) {
+  const float v = (float)acc * sw[0] * sx;
+  if constexpr (PLANES == 1) return v;
+  return v / (1.0f + __expf(-v)) * ((float)acc_up * sw[PLANES - 1] * sx);
+}
+
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_constant__ I8Tc t) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kI8MaxStages], empty[kI8MaxStages], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_base_sh;
   __shared__ int last_sh;
+  __shared__ float sx_sh[2][256];
   uint8_t* ring = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int stage_bytes = PLANES * kChTile * kKBlock + t.bn * kKBlock;
@@ -185,6 +299,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
+  pdl_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -201,16 +316,18 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         tma_load_2d(ring + stage * stage_bytes + PLANES * kChTile * kKBlock, &t.mx, k * kKBlock,
                     s.tile % t.tok_tiles * t.bn, &full[stage]);
       };
-      // The first stages' weights do not depend on the launch before this one.
+      // Behind the quantiser the first stages' weights are asked for at once:
+      // it does not write them, and what came before it is complete.
+      if (!t.after_quantiser) pdl_wait();
       I8Seg s;
       s.begin(t);
       int issued = 0;
-      while (issued < t.stages && s.next(t))
+      while (t.after_quantiser && issued < t.stages && s.next(t))
         for (int k = s.k0; k < s.k1 && issued < t.stages; ++k, ++issued) {
           mbar_arrive_expect_tx(&full[issued], stage_bytes);
           load_w(issued, s, k);
         }
-      pdl_wait();
+      if (t.after_quantiser) pdl_wait();
       s.begin(t);
       int i = 0;  // k blocks so far
       bool ok = true;
@@ -218,7 +335,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         for (int k = s.k0; k < s.k1; ++k, ++i) {
           const int stage = i % t.stages;
           if (i >= issued) {
-            if (!mbar_wait_bounded(&empty[stage], (i / t.stages - 1) & 1)) {
+            if (i >= t.stages && !mbar_wait_bounded(&empty[stage], (i / t.stages - 1) & 1)) {
               *t.error = kErrEmptyWait;
               ok = false;
               break;
@@ -289,21 +406,51 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
       const int buf = n & 1;
       const int tok0 = s.tile % t.tok_tiles * t.bn, j = s.tile / t.tok_tiles * kChTile + ch;
       const int cols = min(t.bn, p.m - tok0);
-      const bool split = s.k0 != 0 || s.k1 != t.kb;
+      const bool split = t.cluster == 1 && (s.k0 != 0 || s.k1 != t.kb);
       float sw[PLANES];
 #pragma unroll
       for (int pl = 0; pl < PLANES; ++pl) sw[pl] = j < p.n ? p.sw[pl * p.n + j] : 0.f;
+      // Everything the epilogue reads from global memory is asked for before
+      // the accumulator is waited for (residual rows: a chunk ahead).
+      float* sx = sx_sh[n & 1];
+      for (int c = et; c < cols; c += 128) sx[c] = p.sx[tok0 + c];
+      const T* res_col = p.residual && j < p.n ? static_cast<const T*>(p.residual) + tok0 * p.ldr + j : nullptr;
+      T res[32];
+      auto load_residual = [&](int c0) {
+        if (!res_col) return;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) res[c] = res_col[min(c0 + c, cols - 1) * p.ldr];
+      };
+      if (t.cluster == 1) load_residual(0);
+      named_sync(1, 128);
       if (!mbar_wait_bounded(&acc_full[buf], (n >> 1) & 1)) {
         *t.error = kErrFullWait;
         break;
       }
       tc_fence_after();
-      int c_first = 0, c_last = 0;
+      // Columns go 32 at a time; those behind the last row are read (scratch or
+      // a clamped row) and not stored, so that no load waits on a branch.
       bool finish = true;
+      int* sums = nullptr;
+      if (t.cluster > 1) {
+        // The ring is free: every MMA that read it is done.  [plane][column][channel].
+        int* mine = reinterpret_cast<int*>(ring);
+        for (int c0 = 0; c0 < cols; c0 += 32) {
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl) {
+            uint32_t r[32];
+            tmem_ld32(lane_addr + (buf * PLANES + pl) * t.bn + c0, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) mine[(pl * t.bn + c0 + c) * kChTile + ch] = (int)r[c];
+          }
+        }
+        break;  // the only segment; the rest is behind the cluster's barrier
+      }
       if (split) {
-        c_first = i8_owner(t, (long long)s.tile * t.kb);
-        c_last = i8_owner(t, (long long)(s.tile + 1) * t.kb - 1);
-        int* mine = t.partials + ((long long)blockIdx.x * 2 + (n > 0)) * t.slot_ints;
+        const int c_first = i8_owner(t, (long long)s.tile * t.kb);
+        const int c_last = i8_owner(t, (long long)(s.tile + 1) * t.kb - 1);
+        sums = t.partials + c_first * t.slot_ints + ch;
         for (int c0 = 0; c0 < cols; c0 += 32) {
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl) {
@@ -312,7 +459,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 32; ++c)
-              if (c0 + c < cols) __stcg(mine + (pl * t.bn + c0 + c) * kChTile + ch, (int)r[c]);
+              if (c0 + c < cols) atomicAdd(sums + (pl * t.bn + c0 + c) * kChTile, (int)r[c]);
           }
         }
         __threadfence();
@@ -329,36 +476,36 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
       if (finish) {
         for (int c0 = 0; c0 < cols; c0 += 32) {
           uint32_t r[PLANES][32];
-#pragma unroll
-          for (int pl = 0; pl < PLANES; ++pl) tmem_ld32(lane_addr + (buf * PLANES + pl) * t.bn + c0, r[pl]);
-          tmem_wait_ld();
+          const int rows = cols - c0;  // of this chunk, if less than 32
           if (split) {
-            for (int c = c_first; c <= c_last; ++c) {
-              if (c == (int)blockIdx.x) continue;
-              // Its first range unless it began before this tile.
-              const int which = c * t.units / gridDim.x / t.kb != s.tile;
-              const int* from = t.partials + ((long long)c * 2 + which) * t.slot_ints;
 #pragma unroll
-              for (int pl = 0; pl < PLANES; ++pl)
+            for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
-                for (int cc = 0; cc < 32; ++cc)
-                  if (c0 + cc < cols) r[pl][cc] += __ldcg(from + (pl * t.bn + c0 + cc) * kChTile + ch);
-            }
+              for (int c = 0; c < 32; ++c) r[pl][c] = __ldcg(sums + (pl * t.bn + c0 + c) * kChTile);
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl)
+#pragma unroll
+              for (int c = 0; c < 32; ++c) __stcg(sums + (pl * t.bn + c0 + c) * kChTile, 0);
+          } else {
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) tmem_ld32(lane_addr + (buf * PLANES + pl) * t.bn + c0, r[pl]);
+            tmem_wait_ld();
           }
+          T* to = static_cast<T*>(p.y) + (tok0 + c0) * p.ldy + j;
+          T out[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            float v = i8_value<PLANES>((int)r[0][c], (int)r[PLANES - 1][c], sw, sx[c0 + c]);
+            if (res_col) v += Act<T>::to_float(res[c]);
+            out[c] = Act<T>::from_float(v);
+          }
+          // Loaded before the stores: residual and y may be one buffer, but a
+          // chunk's rows are its own.
+          load_residual(c0 + 32);
           if (j < p.n) {
 #pragma unroll
-            for (int cc = 0; cc < 32; ++cc) {
-              if (c0 + cc >= cols) break;
-              const int i = tok0 + c0 + cc;
-              const float sx = p.sx[i];
-              float v = (float)(int)r[0][cc] * sw[0] * sx;
-              if constexpr (PLANES == 2) {
-                const float u = (float)(int)r[1][cc] * sw[1] * sx;
-                v = v / (1.0f + __expf(-v)) * u;
-              }
-              if (p.residual) v += Act<T>::to_float(static_cast<const T*>(p.residual)[i * p.ldr + j]);
-              static_cast<T*>(p.y)[i * p.ldy + j] = Act<T>::from_float(v);
-            }
+            for (int c = 0; c < 32; ++c)
+              if (c < rows) to[c * p.ldy] = out[c];
           }
         }
       }
@@ -368,6 +515,60 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
     }
   }
   __syncwarp();
+  if (t.cluster > 1) {
+    // This CTA's columns of the tile, from all the cluster's sums.  What comes
+    // from global memory is asked for before the barrier.
+    const I8Params& p = t.p;
+    const int rank = blockIdx.x % t.cluster, tile = blockIdx.x / t.cluster;
+    const int ch = (warp & 3) * 32 + lane, j = tile / t.tok_tiles * kChTile + ch;
+    const int tok0 = tile % t.tok_tiles * t.bn, cols = min(t.bn, p.m - tok0);
+    const int c_begin = rank * cols / t.cluster, c_end = (rank + 1) * cols / t.cluster;
+    const bool mine = warp >= 2 && j < p.n;
+    constexpr int C = 16;  // columns at a time
+    float sw[PLANES];
+    T res[C];
+    auto load_residual = [&](int c0) {
+      if (!mine || !p.residual) return;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        res[c] = static_cast<const T*>(p.residual)[(long long)(tok0 + max(min(c0 + c, c_end - 1), 0)) * p.ldr + j];
+    };
+#pragma unroll
+    for (int pl = 0; pl < PLANES; ++pl) sw[pl] = mine ? p.sw[pl * p.n + j] : 0.f;
+    load_residual(c_begin);
+    cluster_sync();
+    if (warp >= 2) {
+      const uint32_t sums = smem_addr(ring) + ch * 4;
+      for (int c0 = c_begin; c0 < c_end; c0 += C) {
+        const int n = min(C, c_end - c0);
+        int acc[PLANES][C] = {};
+        for (int peer = 0; peer < t.cluster; ++peer) {
+          const uint32_t from = cluster_map(sums, peer);
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+              acc[pl][c] += ld_cluster(from + (pl * t.bn + c0 + min(c, n - 1)) * kChTile * 4);
+        }
+        T out[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float v = i8_value<PLANES>(acc[0][c], acc[PLANES - 1][c], sw, sx_sh[0][c0 + min(c, n - 1)]);
+          if (p.residual) v += Act<T>::to_float(res[c]);
+          out[c] = Act<T>::from_float(v);
+        }
+        load_residual(c0 + C);
+        if (mine) {
+          T* to = static_cast<T*>(p.y) + (long long)(tok0 + c0) * p.ldy + j;
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+            if (c < n) to[c * p.ldy] = out[c];
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // peers may still be reading this CTA's sums
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -413,29 +614,22 @@ int i8_bn(int m, int planes) {
 }
 
 template <typename T, int PLANES>
-cudaError_t launch_product(const I8Tc& t, int grid, int smem, bool pdl, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(i8_product_kernel<T, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kI8SmemBytes);
+cudaError_t launch_product(const I8Tc& t, int grid, int smem, cudaStream_t stream) {
+  static std::atomic<uint64_t> allowed{0};  // devices whose limit is set
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(i8_product_kernel<T, PLANES>), kI8SmemBytes, &allowed);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kI8Threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, i8_product_kernel<T, PLANES>, t);
+  return launch_after(i8_product_kernel<T, PLANES>, dim3(grid), dim3(kI8Threads), smem, t.cluster, stream, t);
 }
 
 }  // namespace
 
 cudaError_t launch_i8_quantize_rows(const I8RowsParams& p, cudaStream_t stream) {
-  if (p.bf16) quantize_rows_kernel<__nv_bfloat16><<<p.m, 256, 0, stream>>>(p);
-  else quantize_rows_kernel<__half><<<p.m, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  // Four 16-byte loads a thread, 64 to 512 threads.
+  const int threads = std::min(512, std::max(64, (p.k + 1023) / 1024 * 32));
+  void (*kernel)(I8RowsParams) =
+      p.bf16 ? (p.rmsnorm ? quantize_rows_kernel<__nv_bfloat16, true> : quantize_rows_kernel<__nv_bfloat16, false>)
+             : (p.rmsnorm ? quantize_rows_kernel<__half, true> : quantize_rows_kernel<__half, false>);
+  return launch_after(kernel, dim3(p.m), dim3(threads), 0, 1, stream, p);
 }
 
 cudaError_t launch_i8_quantize_weights(const void* w, int K, int N, int layout, int bf16, int8_t* codes,
@@ -453,18 +647,17 @@ cudaError_t launch_i8_quantize_weights(const void* w, int K, int N, int layout, 
 size_t i8_partial_bytes(int max_m, int planes, int num_sms) {
   const int most = 256 / planes;
   const int bn = max_m <= most ? up32(max_m) : most;
-  return (size_t)num_sms * 2 * planes * bn * kChTile * 4;
+  return (size_t)num_sms * planes * bn * kChTile * 4;
 }
 
-cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int* partials, int* error, bool pdl,
-                              cudaStream_t stream) {
+cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int* partials, int* error,
+                              bool after_quantiser, cudaStream_t stream) {
   I8Tc t;
   t.p = p;
   t.bn = i8_bn(p.m, p.planes);
   const int stage_bytes = (p.planes * kChTile + t.bn) * kKBlock;
-  t.stages = kI8SmemBytes / stage_bytes;
-  if (t.stages > kI8MaxStages) t.stages = kI8MaxStages;
-  while (t.stages * stage_bytes + 1024 > kI8SmemBytes) --t.stages;
+  t.stages = std::min(kI8MaxStages, (kI8SmemBytes - 1024) / stage_bytes);
+  if (t.bn * p.planes <= 64 && t.stages * stage_bytes > 100 * 1024) t.stages = 100 * 1024 / stage_bytes;
   t.kb = (p.k + kKBlock - 1) / kKBlock;
   t.tok_tiles = (p.m + t.bn - 1) / t.bn;
   t.tiles = t.tok_tiles * ((p.n + kChTile - 1) / kChTile);
@@ -478,16 +671,23 @@ cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int
   // Whole tiles where the last wave leaves at most a tenth of the SMs' time idle.
   const int waves = (t.tiles + num_sms - 1) / num_sms;
   t.whole = t.tiles * 10LL >= (long long)waves * num_sms * 9;
-  const int grid = t.whole ? (t.tiles < num_sms ? t.tiles : num_sms) : (int)(t.units < num_sms ? t.units : num_sms);
+  int grid = (int)std::min<long long>(t.whole ? t.tiles : t.units, num_sms);
+  // A cluster a tile where at least two CTAs fit for every tile (a GPC holds
+  // 16 SMs or more, so sizes up to 8 pack without much loss).
+  t.cluster = 1;
+  while (!t.whole && t.cluster < 8 && t.tiles * t.cluster * 2 <= num_sms * 9 / 10 && t.cluster * 2 <= t.kb)
+    t.cluster *= 2;
+  if (t.cluster > 1) grid = t.tiles * t.cluster;
+  t.after_quantiser = after_quantiser;
   if (!encode_rows(&t.mw, p.w, (long long)p.planes * p.n, p.k, p.ldw, kChTile) ||
       !encode_rows(&t.mx, p.x, p.m, p.k, p.ldx, t.bn))
     return cudaErrorInvalidValue;
   const int smem = t.stages * stage_bytes + 1024;
   if (p.bf16)
-    return p.planes == 2 ? launch_product<__nv_bfloat16, 2>(t, grid, smem, pdl, stream)
-                         : launch_product<__nv_bfloat16, 1>(t, grid, smem, pdl, stream);
-  return p.planes == 2 ? launch_product<__half, 2>(t, grid, smem, pdl, stream)
-                       : launch_product<__half, 1>(t, grid, smem, pdl, stream);
+    return p.planes == 2 ? launch_product<__nv_bfloat16, 2>(t, grid, smem, stream)
+                         : launch_product<__nv_bfloat16, 1>(t, grid, smem, stream);
+  return p.planes == 2 ? launch_product<__half, 2>(t, grid, smem, stream)
+                       : launch_product<__half, 1>(t, grid, smem, stream);
 }
 
 }  // namespace b2g

@@ -2,6 +2,7 @@
 // kernels of the 8-bit integer product (i8.cu), the cache append
 // (kv_append.cu) and the attention over the cache (attention.cu).
 #pragma once
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -13,6 +14,19 @@ namespace b2g {
 // api.cpp: this device's error word, registered so that b2g_device_error
 // finds it (NULL: no such device, or a CUDA error).
 int* registered_error_word(int dev);
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device,
+// once per device (`done` has a bit for each).
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done->fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 // ---------------------------------------------------------------------------
 // i8.cu
@@ -46,10 +60,11 @@ struct I8Params {
 };
 // Bytes of the split tiles' partial sums for calls of up to max_m rows.
 size_t i8_partial_bytes(int max_m, int planes, int num_sms);
-// counters: [num_sms] zeros, left zero.  pdl: the launch before this one in
-// the stream is the quantiser of p.x (the weights may be read before it ends).
-cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int* partials, int* error, bool pdl,
-                              cudaStream_t stream);
+// counters: [num_sms] zeros, left zero.  after_quantiser: the launch before
+// this one in the stream is the quantiser of p.x (the weights may be read
+// before it ends).
+cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int* partials, int* error,
+                              bool after_quantiser, cudaStream_t stream);
 
 // ---------------------------------------------------------------------------
 // kv_append.cu, attention.cu

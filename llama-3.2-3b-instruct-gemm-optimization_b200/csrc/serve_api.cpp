@@ -9,7 +9,7 @@ using namespace b2g;
 struct b2g_i8_op {
   b2g_i8_fields f;
   int planes, device, num_sms;
-  size_t off_codes, off_scales, off_partials, bytes;  // workspace: counters, codes, scales, partials
+  size_t off_codes, off_scales, off_partials, bytes;  // workspace: counters, codes, scales, split tiles' sums
   long long ld_codes;
 };
 
@@ -155,7 +155,7 @@ b2g_status b2g_i8_workspace_size(const b2g_i8_op* op, size_t* bytes) {
 
 b2g_status b2g_i8_workspace_init(const b2g_i8_op* op, void* ws, b2g_stream_t stream) {
   if (!op || !ws || !aligned(ws, 256)) return B2G_ERR_INVALID;
-  return cuda_status(cudaMemsetAsync(ws, 0, op->off_codes, cu(stream)));
+  return cuda_status(cudaMemsetAsync(ws, 0, op->bytes, cu(stream)));
 }
 
 b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* a, b2g_stream_t stream) {
