@@ -1,0 +1,505 @@
+// attn_rows.cuh -- attention of few rows a k/v head (decode steps, drafts):
+// bound by reading the cache once.
+//
+// A block of four warps walks its share of the work list in units of 64
+// cached tokens, 16 a warp.  Each warp streams its own tokens' keys and
+// values through its own ring of shared memory with 16-byte asynchronous
+// copies (page by page, nothing shared, so no barrier in the loop), and keeps
+// its own running maximum, sum and output for the 16 rows of the tile in
+// m16n8k16 fragments.  At the end of an item the warps' parts are joined in
+// shared memory, and the blocks' parts of a split item by the last block to
+// arrive, always in the same order.
+#pragma once
+#include <type_traits>
+
+#include "serve.cuh"
+
+namespace b2g {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^x to 2^-22 of its value; 0 for -infinity and below 2^-126.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma_act(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    mma_16816(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 bytes global -> shared, zeros where !in (src is not read then).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// T: the activations' type.  With an 8-bit cache the products run in fp16
+// (every E4M3 value is one): bf16 rows of q are brought into its range by a
+// power of two each.
+template <typename T, bool FP8, int D>
+struct RowsKernel {
+  static constexpr int kRows = 16, kUnit = 64, kWarps = 4;
+  static constexpr bool kBf16 = !FP8 && sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
+  static constexpr int kTileBytes = 16 * kRowBytes;       // 16 tokens of keys or values
+  static constexpr int kStageBytes = 2 * kTileBytes;      // of one warp
+  static constexpr int kStages = 24576 / kStageBytes;     // 24 KB a warp in flight
+  static constexpr int kNT = D / 8;                       // output tiles of 8 columns
+  static constexpr int kSmem = kWarps * kStages * kStageBytes + kNT * 32 * 16;
+  static constexpr int kPartFloats = kNT * 32 * 4 + 32;   // a part: fragments, then maximum and sum of 16 rows
+
+  using Work = AttnWork<kRows, kUnit>;
+
+  // 16-byte chunk of a token's row inside its tile.  Sixteen or eight chunks
+  // a row: eight consecutive tokens' same chunk lie in different banks.
+  static __device__ __forceinline__ uint32_t chunk_at(int token, int c) {
+    if constexpr (kRowBytes == 64) return token * 64 + ((c ^ ((token >> 1) & 3)) * 16);
+    if constexpr (FP8) return token * kRowBytes + ((c ^ (((token & 1) << 2) | ((token >> 1) & 3))) * 16);
+    return token * kRowBytes + ((c ^ (token & 7)) * 16);
+  }
+
+  // Column of element e (0, 1) of output tile j for lane quarter q.
+  static __device__ __forceinline__ int column(int j, int q, int e) {
+    if constexpr (FP8) return 16 * (j / 2) + 4 * q + 2 * e + (j & 1);
+    return 8 * j + 2 * q + e;
+  }
+
+  static __device__ void run(const AttnParams& p);
+};
+
+template <typename T, bool FP8, int D>
+__device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ long long sh[8];
+  __shared__ float sh_ml[2][16];
+  __shared__ int sh_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const uint32_t ring = smem_addr(smem) + warp * kStages * kStageBytes;
+  float* join = reinterpret_cast<float*>(smem + kWarps * kStages * kStageBytes);
+  pdl_wait();
+  pdl_launch_dependents();
+  const Work w(p);
+  const AttnShare share = attn_share(w, p.least_units, sh);
+  if (share.begin >= share.end) return;
+
+  // The stream of units: where the copies are, ahead of the products.
+  long long at0 = share.at;
+  AttnItem pi = w.find(share.b, at0);
+  int pu = pi.u_lo + (int)at0;
+  long long left = share.end - share.begin;  // units not yet asked for
+  long long row_at = 0;                      // lanes 0..15: a token's row in the cache, -1: none
+  auto look_up = [&]() {
+    if (left <= 0) return;
+    const int j = pu * kUnit + warp * 16 + (lane & 15);
+    row_at = -1;
+    if (j >= pi.lo && j < pi.hi) {
+      const int pg = j / p.c.page_size;
+      const int page = page_of(p.b, p.c, pi.b, pg, p.error);
+      if (page >= 0)
+        row_at = page * p.c.stride_page + (long long)(j - pg * p.c.page_size) * p.c.stride_token +
+                 pi.h * p.c.stride_head;
+    }
+  };
+  uint32_t seen[kStages];  // bit t: the stage's token t is there
+  const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
+  const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
+  auto copy = [&](uint32_t dst) -> uint32_t {
+    uint32_t mask = 0;
+    if (left > 0) {
+      constexpr int kChunks = kRowBytes / 16, kPerPass = 32 / kChunks;  // tokens a pass of the lanes
+      const int c = lane % kChunks;
+#pragma unroll
+      for (int i = 0; i < 16 / kPerPass; ++i) {
+        const int t = i * kPerPass + lane / kChunks;
+        const long long row = __shfl_sync(0xffffffffu, row_at, t);
+        const bool in = row >= 0;
+        const long long off = in ? row * (FP8 ? 1 : 2) + c * 16 : 0;
+        cp_async16_or_zero(dst + chunk_at(t, c), kb + off, in);
+        cp_async16_or_zero(dst + kTileBytes + chunk_at(t, c), vb + off, in);
+      }
+      mask = __ballot_sync(0xffffffffu, row_at >= 0) & 0xffff;
+      --left;
+      if (++pu == pi.u_hi && left > 0) {
+        w.next(pi);
+        pu = pi.u_lo;
+      }
+    }
+    cp_async_commit();
+    return mask;
+  };
+  look_up();
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    seen[i] = copy(ring + i * kStageBytes);
+    look_up();
+  }
+  seen[kStages - 1] = 0;
+
+  // The products.
+  at0 = share.at;
+  AttnItem it = w.find(share.b, at0);
+  long long pos = share.begin;  // units done
+  int stage = 0;
+  for (;;) {
+    const int u0 = it.u_lo + (int)at0;
+    const long long item_begin = pos - at0;
+    const int units = (int)min((long long)(it.u_hi - u0), share.end - pos);
+    const bool split = units != it.u_hi - it.u_lo;
+    // q as A fragments, scaled into fp16's range where the cache is 8-bit.
+    const int rows = it.s.n * p.group;
+    uint32_t qf[D / 16][4];
+    float q_mul[2];
+    int row_pos[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = it.tile * kRows + g + 8 * hf;
+      const int i = r / p.group;
+      const bool in = r < rows;
+      row_pos[hf] = in ? it.s.ctx + i : -1;
+      const T* src = static_cast<const T*>(p.a.q) + (long long)(it.s.first + i) * p.a.stride_q +
+                     (it.h * p.group + r - i * p.group) * p.a.stride_q_head;
+      float amax = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // Elements of k slots 2q, 2q + 1 (half 0) and 8 + 2q, 9 + 2q (half 1).
+          // 8-bit: D / 4 consecutive elements a lane in two runs (see below).
+          const int d = FP8 ? (D == 128 ? (s / 4) * 64 + q4 * 16 + (s % 4) * 4 + 2 * half
+                                        : q4 * 16 + s * 4 + 2 * half)
+                            : 16 * s + 8 * half + 2 * q4;
+          uint32_t v = in ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+          qf[s][half * 2 + hf] = v;
+          if constexpr (FP8 && std::is_same<T, __nv_bfloat16>::value) {
+            const float2 f = Act<T>::unpack(v);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+      }
+      q_mul[hf] = 1.0f;
+      if constexpr (FP8 && std::is_same<T, __nv_bfloat16>::value) {
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int e = (int)(__float_as_uint(amax) >> 23);  // amax = 2^(e - 127) * 1.x
+        float up = 1.0f;
+        if (e > 0 && e < 255) {
+          up = __uint_as_float((uint32_t)min(max(127 + 13 - (e - 127), 1), 253) << 23);
+          q_mul[hf] = 1.0f / up;
+        }
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float2 f = Act<T>::unpack(qf[s][half * 2 + hf]);
+            qf[s][half * 2 + hf] = Act<__half>::pack(f.x * up, f.y * up);
+          }
+      }
+    }
+    const float ks = FP8 && p.c.k_scale ? p.c.k_scale[it.h] : 1.0f;
+    const float scale[2] = {p.a.scale * kLog2e * ks * q_mul[0], p.a.scale * kLog2e * ks * q_mul[1]};
+    const int low[2] = {p.a.window > 0 ? row_pos[0] - p.a.window : -1, p.a.window > 0 ? row_pos[1] - p.a.window : -1};
+
+    float o[kNT][4];
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int n = 0; n < units; ++n) {
+      // The stage that was read last is free: ask for the next unit.
+      {
+        const int to = stage == 0 ? kStages - 1 : stage - 1;
+        const uint32_t mask = copy(ring + to * kStageBytes);
+#pragma unroll
+        for (int i = 0; i < kStages; ++i)
+          if (i == to) seen[i] = mask;
+        look_up();
+      }
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      uint32_t here = 0;
+#pragma unroll
+      for (int i = 0; i < kStages; ++i)
+        if (i == stage) here = seen[i];
+      const uint32_t kt = ring + stage * kStageBytes, vt = kt + kTileBytes;
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      if (here != 0) {
+        float s[2][4] = {};
+        if constexpr (!FP8) {
+          // Matrices: tokens 0-7 / 8-15 by d halves of a k16 step.
+          const int t = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+          for (int ss = 0; ss < D / 16; ++ss) {
+            uint32_t b[4];
+            ldsm4(b, kt + chunk_at(t, 2 * ss + half));
+            mma_act<kBf16>(s[0], qf[ss], b[0], b[1]);
+            mma_act<kBf16>(s[1], qf[ss], b[2], b[3]);
+          }
+        } else {
+          // A product over d may take d in any order: lane quarter q takes the
+          // 16 bytes q (and 4 + q) of a token, four k16 steps of 2 + 2.
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int hf = 0; hf < D / 64; ++hf) {
+              const uint4 v = lds128_at(kt + chunk_at(nt * 8 + g, hf * 4 + q4));
+              const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t b0, b1;
+                e4m3x4_to_f16x2x2(wd[i], b0, b1);
+                mma_act<false>(s[nt], qf[hf * 4 + i], b0, b1);
+              }
+            }
+        }
+        // Scores of rows g, g + 8 and tokens 8 nt + 2q, + 1.
+        const int j0 = (u0 + n) * kUnit + warp * 16;
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = nt * 8 + 2 * q4 + (e & 1), j = j0 + t, hf = e >> 1;
+            const bool sees = j <= row_pos[hf] && j > low[hf] && (here >> t & 1);
+            s[nt][e] = sees ? s[nt][e] * scale[hf] : -INFINITY;
+            mx[hf] = fmaxf(mx[hf], s[nt][e]);
+          }
+        float al[2];
+        bool same = true;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+          const float mn = fmaxf(m[hf], mx[hf]);
+          const float base = mn == -INFINITY ? 0.f : mn;
+          al[hf] = exp2_fast(m[hf] - base);
+          same = same && m[hf] == mn;
+          m[hf] = mn;
+          mx[hf] = base;
+        }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = exp2_fast(s[nt][e] - mx[e >> 1]);
+        if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) l[hf] *= al[hf];
+#pragma unroll
+          for (int j = 0; j < kNT; ++j) {
+            o[j][0] *= al[0];
+            o[j][1] *= al[0];
+            o[j][2] *= al[1];
+            o[j][3] *= al[1];
+          }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          l[hf] += (s[0][2 * hf] + s[0][2 * hf + 1]) + (s[1][2 * hf] + s[1][2 * hf + 1]);
+        using P = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
+        const uint32_t pf[4] = {Act<P>::pack(s[0][0], s[0][1]), Act<P>::pack(s[0][2], s[0][3]),
+                                Act<P>::pack(s[1][0], s[1][1]), Act<P>::pack(s[1][2], s[1][3])};
+        // Values: matrices of tokens 0-7 / 8-15 by 16-byte chunks, transposed.
+        const int t = lane & 15, half = lane >> 4;
+#pragma unroll
+        for (int c = 0; c < kRowBytes / 16; c += 2) {
+          uint32_t b[4];
+          ldsm4_t(b, vt + chunk_at(t, c + half));
+          if constexpr (!FP8) {
+            mma_act<kBf16>(o[c], pf, b[0], b[1]);
+            mma_act<kBf16>(o[c + 1], pf, b[2], b[3]);
+          } else {
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              // Bytes: token 2q (d 2n, 2n + 1), token 2q + 1 (the same d).
+              uint32_t e0, o0, e1, o1;
+              e4m3x4_to_f16x2x2(__byte_perm(b[2 * cc], 0, 0x3120), e0, o0);
+              e4m3x4_to_f16x2x2(__byte_perm(b[2 * cc + 1], 0, 0x3120), e1, o1);
+              mma_act<false>(o[2 * (c + cc)], pf, e0, e1);
+              mma_act<false>(o[2 * (c + cc) + 1], pf, o0, o1);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+    pos += units;
+
+    // The warps' parts, into warp 0's.
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+    }
+    float4* jo = reinterpret_cast<float4*>(join);
+    for (int from = 1; from < kWarps; ++from) {
+      if (warp == from) {
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) jo[j * 32 + lane] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+        if (q4 == 0) {
+          sh_ml[0][g] = m[0];
+          sh_ml[0][g + 8] = m[1];
+          sh_ml[1][g] = l[0];
+          sh_ml[1][g + 8] = l[1];
+        }
+      }
+      __syncthreads();
+      if (warp == 0) {
+        float a[2], b[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float mo = sh_ml[0][g + 8 * hf];
+          const float mn = fmaxf(m[hf], mo), base = mn == -INFINITY ? 0.f : mn;
+          a[hf] = exp2_fast(m[hf] - base);
+          b[hf] = exp2_fast(mo - base);
+          l[hf] = l[hf] * a[hf] + sh_ml[1][g + 8 * hf] * b[hf];
+          m[hf] = mn;
+        }
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          const float4 v = jo[j * 32 + lane];
+          o[j][0] = o[j][0] * a[0] + v.x * b[0];
+          o[j][1] = o[j][1] * a[0] + v.y * b[0];
+          o[j][2] = o[j][2] * a[1] + v.z * b[1];
+          o[j][3] = o[j][3] * a[1] + v.w * b[1];
+        }
+      }
+      __syncthreads();
+    }
+    const float vs = FP8 && p.c.v_scale ? p.c.v_scale[it.h] : 1.0f;
+    auto write = [&](int hf, float mm, float ll, auto value, int j_from, int j_to) {
+      const int r = it.tile * kRows + g + 8 * hf;
+      if (r >= rows) return;
+      const int i = r / p.group, h = it.h * p.group + r - i * p.group;
+      const long long t = it.s.first + i;
+      const float inv = ll == 0.f ? 0.f : vs / ll;
+      T* out = static_cast<T*>(p.a.out) + t * p.a.stride_o + h * p.a.stride_o_head;
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        if (j < j_from || j >= j_to) continue;
+        if constexpr (FP8) {
+          if (j & 1) continue;  // tiles j, j + 1 interleave: four consecutive columns
+          uint2 v;
+          v.x = Act<T>::pack(value(j, 2 * hf) * inv, value(j + 1, 2 * hf) * inv);
+          v.y = Act<T>::pack(value(j, 2 * hf + 1) * inv, value(j + 1, 2 * hf + 1) * inv);
+          *reinterpret_cast<uint2*>(out + column(j, q4, 0)) = v;
+        } else {
+          *reinterpret_cast<uint32_t*>(out + column(j, q4, 0)) =
+              Act<T>::pack(value(j, 2 * hf) * inv, value(j, 2 * hf + 1) * inv);
+        }
+      }
+      if (p.a.lse && q4 == 0 && j_from == 0)
+        p.a.lse[t * p.q_heads + h] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) / kLog2e;
+    };
+    if (!split) {
+      if (warp == 0)
+        for (int hf = 0; hf < 2; ++hf) write(hf, m[hf], l[hf], [&](int j, int e) { return o[j][e]; }, 0, kNT);
+    } else {
+      // This block's part, and the join by the last block to arrive.
+      float* parts = static_cast<float*>(p.parts);
+      const int c_first = attn_owner(share, item_begin);
+      const int c_last = attn_owner(share, item_begin + (it.u_hi - it.u_lo) - 1);
+      if (warp == 0) {
+        float* mine = parts + ((long long)blockIdx.x * 2 + (pos - units != share.begin)) * kPartFloats;
+        float4* po = reinterpret_cast<float4*>(mine);
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) __stcg(po + j * 32 + lane, make_float4(o[j][0], o[j][1], o[j][2], o[j][3]));
+        if (q4 == 0) {
+          float* ml = mine + kNT * 32 * 4;
+          __stcg(ml + g, m[0]);
+          __stcg(ml + g + 8, m[1]);
+          __stcg(ml + 16 + g, l[0]);
+          __stcg(ml + 24 + g, l[1]);
+        }
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+          const int n = atom_add_acq_rel_gpu(p.counters + c_first, 1);
+          sh_last = n == c_last - c_first;
+          if (sh_last) p.counters[c_first] = 0;
+        }
+      }
+      __syncthreads();
+      if (sh_last) {
+        __threadfence();
+        auto part = [&](int c) {
+          const bool first = (long long)c * share.total / share.blocks >= item_begin;
+          return parts + ((long long)c * 2 + (first ? 0 : 1)) * kPartFloats;
+        };
+        // Every warp joins a quarter of the columns, in the blocks' order.
+        constexpr int NJ = kNT / kWarps;
+        const bool low_only = rows - it.tile * kRows <= 8;
+        float mm[2] = {-INFINITY, -INFINITY};
+#pragma unroll 4
+        for (int c = c_first; c <= c_last; ++c) {
+          const float* ml = part(c) + kNT * 32 * 4;
+          mm[0] = fmaxf(mm[0], __ldcg(ml + g));
+          mm[1] = fmaxf(mm[1], __ldcg(ml + g + 8));
+        }
+        const float base[2] = {mm[0] == -INFINITY ? 0.f : mm[0], mm[1] == -INFINITY ? 0.f : mm[1]};
+        float ll[2] = {0.f, 0.f}, acc[NJ][4] = {};
+#pragma unroll 4
+        for (int c = c_first; c <= c_last; ++c) {
+          const float* ml = part(c) + kNT * 32 * 4;
+          const float a0 = exp2_fast(__ldcg(ml + g) - base[0]), a1 = exp2_fast(__ldcg(ml + g + 8) - base[1]);
+          ll[0] += __ldcg(ml + 16 + g) * a0;
+          ll[1] += __ldcg(ml + 24 + g) * a1;
+          const float4* po = reinterpret_cast<const float4*>(part(c)) + warp * NJ * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            const float4 v = __ldcg(po + j * 32);
+            acc[j][0] += v.x * a0;
+            acc[j][1] += v.y * a0;
+            acc[j][2] += v.z * a1;
+            acc[j][3] += v.w * a1;
+          }
+        }
+        for (int hf = 0; hf < (low_only ? 1 : 2); ++hf)
+          write(hf, mm[hf], ll[hf],
+                [&](int j, int e) {
+                  float v = 0.f;
+#pragma unroll
+                  for (int i = 0; i < NJ; ++i)
+                    if (j == warp * NJ + i) v = acc[i][e];
+                  return v;
+                },
+                warp * NJ, (warp + 1) * NJ);
+      }
+      __syncthreads();
+    }
+    if (pos >= share.end) break;
+    w.next(it);
+    at0 = 0;
+  }
+  cp_async_wait<0>();
+}
+
+template <typename T, bool FP8, int D>
+__global__ void __launch_bounds__(128, 2) attn_rows_kernel(const __grid_constant__ AttnParams p) {
+  RowsKernel<T, FP8, D>::run(p);
+}
+
+}  // namespace b2g

@@ -123,4 +123,145 @@ __device__ __forceinline__ int page_of(const b2g_kv_batch& b, const b2g_kv_cache
   return page;
 }
 
+// ---------------------------------------------------------------------------
+// The attention kernels' work list.  An item is (sequence, tile of rows, k/v
+// head): the rows of a k/v head are its new tokens times its group of q
+// heads, row r being token r / group and head r % group of the group.  An
+// item's visible cached tokens are cut into units of UNIT tokens; the units
+// of all items in order are dealt to the blocks in equal consecutive ranges,
+// so that long contexts, many short ones and ragged mixtures all fill the
+// GPU, from lengths that only the device knows.  A range's first and last
+// item may be shared with other blocks.
+// ---------------------------------------------------------------------------
+struct AttnItem {
+  SeqSpan s;
+  int b, tile, h;
+  int lo, hi;      // visible cached tokens [lo, hi)
+  int u_lo, u_hi;  // units [u_lo, u_hi), at least one
+};
+
+template <int ROWS, int UNIT>
+struct AttnWork {
+  const AttnParams& p;
+  int cap;  // tokens that the page table has entries for
+  __device__ __forceinline__ explicit AttnWork(const AttnParams& p_) : p(p_) {
+    cap = (int)min((long long)p_.b.max_pages * p_.c.page_size, 0x7fffffffLL - UNIT);
+  }
+  __device__ __forceinline__ int tiles(const SeqSpan& s) const { return (s.n * p.group + ROWS - 1) / ROWS; }
+  __device__ __forceinline__ void range(AttnItem& it) const {
+    const int first = it.tile * ROWS / p.group;
+    const int last = min(it.s.n - 1, (it.tile * ROWS + ROWS - 1) / p.group);
+    if (it.s.ctx + last >= cap) *p.error = kErrBadPage;
+    it.hi = max(min(it.s.ctx + last + 1, cap), 0);
+    it.lo = p.a.window > 0 ? min(max(it.s.ctx + first - p.a.window + 1, 0), it.hi) : 0;
+    it.u_lo = it.lo / UNIT;
+    it.u_hi = max((it.hi + UNIT - 1) / UNIT, it.u_lo + 1);
+  }
+  // Units of a sequence's items.
+  __device__ __forceinline__ long long units(int b) const {
+    AttnItem it;
+    it.s = seq_span(p.b, b);
+    long long n = 0;
+    const int nt = tiles(it.s);
+    for (it.tile = 0; it.tile < nt; ++it.tile) {
+      range(it);
+      n += it.u_hi - it.u_lo;
+    }
+    return n * p.c.kv_heads;
+  }
+  // The item that holds unit `at` of sequence b; `at` becomes the unit's
+  // offset in the item.
+  __device__ __forceinline__ AttnItem find(int b, long long& at) const {
+    AttnItem it;
+    it.b = b;
+    it.s = seq_span(p.b, b);
+    for (it.tile = 0;; ++it.tile) {
+      range(it);
+      const long long n = (long long)(it.u_hi - it.u_lo) * p.c.kv_heads;
+      if (at < n) break;
+      at -= n;
+    }
+    it.h = (int)(at / (it.u_hi - it.u_lo));
+    at -= (long long)it.h * (it.u_hi - it.u_lo);
+    return it;
+  }
+  // The next item in order (false: none left).
+  __device__ __forceinline__ bool next(AttnItem& it) const {
+    if (++it.h < p.c.kv_heads) return true;
+    it.h = 0;
+    if (++it.tile < tiles(it.s)) {
+      range(it);
+      return true;
+    }
+    it.tile = 0;
+    while (++it.b < p.b.batch) {
+      it.s = seq_span(p.b, it.b);
+      if (it.s.n > 0) {
+        range(it);
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+// A block's place in the work list.
+struct AttnShare {
+  long long total, begin, end;  // units
+  int blocks;                   // that share the list; others have none
+  int b;                        // the sequence of unit `begin`,
+  long long at;                 // and the unit's offset in it
+};
+
+// Sums the list (all threads; sh: blockDim.x + 1 words) and finds the block's
+// range.  At least `least` units a block, so that short work is not cut finer
+// than the joining of its pieces is worth.
+template <typename Work>
+__device__ __forceinline__ AttnShare attn_share(const Work& w, int least, long long* sh) {
+  const int threads = blockDim.x, batch = w.p.b.batch;
+  const int per = (batch + threads - 1) / threads;
+  const int b0 = min((int)threadIdx.x * per, batch), b1 = min(b0 + per, batch);
+  long long sum = 0;
+  for (int b = b0; b < b1; ++b) sum += w.units(b);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long incl = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off *= 2) {
+    const long long o = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 31) sh[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int i = 0; i < threads / 32; ++i) {
+    if (i < warp) before += sh[i];
+    total += sh[i];
+  }
+  __syncthreads();
+  AttnShare r;
+  r.total = total;
+  r.blocks = (int)max(1LL, min((long long)gridDim.x, (total + least - 1) / least));
+  r.begin = (long long)blockIdx.x * total / r.blocks;
+  r.end = (long long)(blockIdx.x + 1) * total / r.blocks;
+  if ((int)blockIdx.x >= r.blocks) r.begin = r.end = total;
+  // The thread whose sequences hold `begin` tells the others.
+  const long long from = before + incl - sum;
+  if (r.begin >= from && r.begin < from + sum) {
+    long long at = r.begin - from;
+    int b = b0;
+    for (long long n; at >= (n = w.units(b)); ++b) at -= n;
+    sh[0] = b;
+    sh[1] = at;
+  }
+  __syncthreads();
+  r.b = (int)sh[0];
+  r.at = sh[1];
+  __syncthreads();
+  return r;
+}
+// The block that has unit u.
+__device__ __forceinline__ int attn_owner(const AttnShare& s, long long u) {
+  return (int)(((u + 1) * s.blocks - 1) / s.total);
+}
+
 }  // namespace b2g

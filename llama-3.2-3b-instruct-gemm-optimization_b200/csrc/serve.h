@@ -82,8 +82,14 @@ struct AttnParams {
   b2g_kv_cache c;
   b2g_kv_batch b;
   int q_heads, group, bf16;
+  int least_units;  // units of work a block at least
   int* error;
+  int* counters;  // [blocks] zeros, left zero
+  void* parts;    // [blocks][2] parts of split items
 };
-cudaError_t launch_attention(const AttnParams& p, cudaStream_t stream);
+// Bytes of counters and of parts for any call on a device of num_sms SMs.
+size_t attn_counter_bytes(int num_sms);
+size_t attn_part_bytes(int num_sms, int head_dim);
+cudaError_t launch_attention(const AttnParams& p, int num_sms, cudaStream_t stream);
 
 }  // namespace b2g

@@ -16,7 +16,7 @@ struct b2g_i8_op {
 struct b2g_attn {
   b2g_attn_fields f;
   int device, num_sms;
-  size_t bytes;
+  size_t off_parts, bytes;  // workspace: counters, parts of split items
 };
 
 namespace {
@@ -267,7 +267,8 @@ b2g_status b2g_attn_create(const b2g_attn_fields* f, b2g_attn** out) {
   op->f = *f;
   op->device = dev;
   op->num_sms = sms;
-  op->bytes = 256;
+  op->off_parts = attn_counter_bytes(sms);
+  op->bytes = op->off_parts + attn_part_bytes(sms, f->head_dim);
   *out = op;
   return B2G_OK;
 }
@@ -285,7 +286,7 @@ b2g_status b2g_attn_workspace_size(const b2g_attn* op, size_t* bytes) {
 
 b2g_status b2g_attn_workspace_init(const b2g_attn* op, void* ws, b2g_stream_t stream) {
   if (!op || !ws || !aligned(ws, 256)) return B2G_ERR_INVALID;
-  return cuda_status(cudaMemsetAsync(ws, 0, op->bytes, cu(stream)));
+  return cuda_status(cudaMemsetAsync(ws, 0, op->off_parts, cu(stream)));
 }
 
 b2g_status b2g_attn_enqueue(const b2g_attn* op, const b2g_attn_args* a, const b2g_kv_cache* c, const b2g_kv_batch* b,
@@ -315,7 +316,9 @@ b2g_status b2g_attn_enqueue(const b2g_attn* op, const b2g_attn_args* a, const b2
   p.bf16 = op->f.dtype == B2G_DTYPE_BF16;
   p.error = registered_error_word(dev);
   if (!p.error) return B2G_ERR_CUDA;
-  return cuda_status(launch_attention(p, cu(stream)));
+  p.counters = static_cast<int*>(a->workspace);
+  p.parts = static_cast<uint8_t*>(a->workspace) + op->off_parts;
+  return cuda_status(launch_attention(p, op->num_sms, cu(stream)));
 }
 
 }  // extern "C"
