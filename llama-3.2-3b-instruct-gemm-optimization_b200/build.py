@@ -17,7 +17,8 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libb200gemv.so"
 SOURCES = ["gemv.cu", "pack.cu", "static_scratch.cu", "i8.cu", "kv_append.cu", "attention.cu", "api.cpp",
            "serve_api.cpp"]
-HEADERS = ["device.cuh", "gemv.h", "serve.h", "serve.cuh", "tc.cuh", "attn_rows.cuh"]
+HEADERS = ["device.cuh", "gemv.h", "serve.h", "serve.cuh", "tc.cuh", "attn_rows.cuh",
+           "attn_tiles.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -52,6 +52,7 @@ __device__ __forceinline__ int ld_cluster(uint32_t addr) {
 }
 
 constexpr int kErrBadPage = 6;  // a page table entry outside the cache, or a token past the table
+constexpr int kErrAlignment = 7;  // shared memory not placed as a kernel needs it
 
 template <typename T>
 struct Act;
