@@ -19,6 +19,20 @@ cudaError_t launch_rows(AttnParams p, int num_sms, cudaStream_t stream) {
   return launch_after(attn_rows_kernel<T, FP8, D>, dim3(2 * num_sms), dim3(128), K::kSmem, 1, stream, p);
 }
 
+// A 16-bit cache as (dim, row, head, page); loads of 64 elements by `rows`.
+bool encode_cache(CUtensorMap* map, void* base, const b2g_kv_cache& c, int rows) {
+  const EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.kv_heads,
+                              (cuuint64_t)c.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)c.stride_token * 2, (cuuint64_t)c.stride_head * 2,
+                                 (cuuint64_t)c.stride_page * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, bool FP8, int D>
 cudaError_t launch_tiles(AttnParams p, int num_sms, cudaStream_t stream) {
   using K = TilesKernel<T, FP8, D>;
@@ -26,7 +40,19 @@ cudaError_t launch_tiles(AttnParams p, int num_sms, cudaStream_t stream) {
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(attn_tiles_kernel<T, FP8, D>), K::kSmem, &allowed);
   if (e != cudaSuccess) return e;
   p.least_units = 2;
-  return launch_after(attn_tiles_kernel<T, FP8, D>, dim3(num_sms), dim3(K::kThreads), K::kSmem, 1, stream, p);
+  AttnTilesParams a;
+  a.p = p;
+  a.tma.box_rows = 0;
+  // Pages that divide a unit, or that units divide, in 8-row steps (the
+  // swizzle's period): whole units by TMA.  Other pages, 8-bit caches (they
+  // are widened on the way) and strides beyond a tensor map's go by 16-byte
+  // copies.
+  const int page = p.c.page_size;
+  if (!FP8 && page % 8 == 0 && (K::kUnit % page == 0 || page % K::kUnit == 0)) {
+    const int rows = page < K::kUnit ? page : K::kUnit;
+    if (encode_cache(&a.tma.k, p.c.k, p.c, rows) && encode_cache(&a.tma.v, p.c.v, p.c, rows)) a.tma.box_rows = rows;
+  }
+  return launch_after(attn_tiles_kernel<T, FP8, D>, dim3(num_sms), dim3(K::kThreads), K::kSmem, 1, stream, a);
 }
 
 template <typename T, bool FP8, int D>

@@ -3,20 +3,26 @@
 //
 // A persistent block an SM walks its share of the work list in units of 128
 // cached tokens by 256 rows (two tiles of 128, one tcgen05 M each):
-//   warps 0-3, 4-7   softmax of tile 0 and 1: a thread owns a row.  S comes
-//                    from tensor memory, P goes back over it in 16 bits.  The
-//                    running maximum is only moved (and O rescaled in tensor
-//                    memory) once it has grown by 2^8, so P stays in fp16's
-//                    range and most units touch O not at all.
+//   warps 0-3, 4-7   softmax of tile 0 and 1: a thread owns a row.  64 columns
+//                    of S come from tensor memory into registers, P goes back
+//                    over them in 16 bits.  The running maximum is only moved
+//                    (and O rescaled in tensor memory) once it has grown by
+//                    2^8, so P stays in fp16's range and most steps touch O
+//                    not at all.
 //   warps 8-11       keys and values, page by page, into a ring of 128-token
 //                    stages (16-byte asynchronous copies in the 128-byte
 //                    swizzle; an 8-bit cache is widened to fp16 on the way),
 //                    and the rows of q.
-//   warp 12          issues S = Q K^T and O += P V.  While one tile's softmax
-//                    runs, the tensor cores work on the other tile.
-// Tensor memory: S0, S1 (128 columns each), O0, O1 (D columns each).  A tile's
-// S(j + 1) is issued behind its O += P(j) V(j) and one commit covers both, so
-// the softmax warps that see S(j + 1) may touch O.
+//   warps 12, 13     issue S = Q K^T and O += P V of tile 0 and 1 in steps of 64
+//                    tokens.  (Two of them: a wait of theirs stands ~250 clocks
+//                    in line behind the softmax warps' exponentials, and one
+//                    warp's waits are the other's products.)
+// Tensor memory: S0, S1 (two buffers of 64 columns each), O0, O1 (D columns
+// each).  With two buffers the scores of step u + 1 are there when a tile's
+// softmax gets to them, so neither side waits for the other's latency (with
+// one buffer of 128 columns a unit took 4650 clocks, 1800 of them from a P to
+// the next S).  A tile's S(u + 2) is issued behind its O += P(u) V(u) into the
+// same buffer and one commit covers both.
 // Every wait is bounded; after one has run out its thread goes through the
 // remaining steps without waiting, so that barriers still meet.
 #pragma once
@@ -25,24 +31,54 @@
 
 namespace b2g {
 
-template <int N>
-__device__ __forceinline__ void reg_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+// Maximum of three; a NaN stays one.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
-template <int N>
-__device__ __forceinline__ void reg_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+
+// Two floats in one register pair, one instruction for both.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
+__device__ __forceinline__ float2 unpair2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The cache as tensors of (dim, row of a page, head, page) for whole units of
+// pages that a unit is cut into evenly (box_rows rows a load, 0: not so).
+struct AttnTma {
+  CUtensorMap k, v;
+  int box_rows;
+};
+struct AttnTilesParams {
+  AttnParams p;
+  AttnTma tma;
+};
 
 template <typename T, bool FP8, int D>
 struct TilesKernel {
-  static constexpr int kRows = 256, kTile = 128, kUnit = 128, kThreads = 512;
+  static constexpr int kRows = 256, kTile = 128, kUnit = 128, kStep = 64, kThreads = 512;
   static constexpr bool kBf16 = !FP8 && std::is_same<T, __nv_bfloat16>::value;  // the products' type
   static constexpr bool kScaleQ = FP8 && std::is_same<T, __nv_bfloat16>::value;  // bf16 q into fp16's range
   static constexpr int kPanels = D / 64;             // 128-byte panels of a row
   static constexpr int kPanelBytes = kTile * 128;
   static constexpr int kTileBytes = kPanels * kPanelBytes;  // 128 tokens or rows, 16-bit
-  static constexpr int kStages = 4;
+  static constexpr int kStages = FP8 ? 4 : 5;
   static constexpr int kStagingBytes = FP8 ? kTile * D : 0;  // an 8-bit tile
   static constexpr int kOffRing = 2 * kTileBytes, kOffStaging = kOffRing + kStages * kTileBytes;
   static constexpr int kSmem = kOffStaging + 2 * kStagingBytes;
@@ -51,7 +87,7 @@ struct TilesKernel {
   using P16 = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
 
   struct Shared {
-    uint64_t kv_full[kStages], kv_empty[kStages], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain;
+    uint64_t kv_full[kStages], kv_empty[kStages], q_full, q_empty, s_full[2][2], p_full[2][2], drain[2];
     long long share[kThreads / 32];
     long long row_at[2][kTile];  // the unit's tokens' rows in the cache, -1: none
     uint32_t there[8][4];        // bit t: token t of unit (u mod 8) is there
@@ -66,8 +102,8 @@ struct TilesKernel {
     return (c >> 3) * kPanelBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
   }
 
-  static __device__ void load(const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share);
-  static __device__ void multiply(const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share);
+  static __device__ void load(const AttnTma& tma, const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share);
+  static __device__ void multiply(const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share, int t);
   static __device__ void softmax(const AttnParams& p, Shared& s, const AttnShare& share, int tile);
 };
 
@@ -106,17 +142,18 @@ struct AttnWalk {
 // Loads
 // ---------------------------------------------------------------------------
 template <typename T, bool FP8, int D>
-__device__ void TilesKernel<T, FP8, D>::load(const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share) {
+__device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share) {
   const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5;
   const Work w(p);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok && !mbar_wait_bounded(bar, parity)) {
+    if (ok && !mbar_wait_spin(bar, parity)) {
       *p.error = kErrEmptyWait;
       ok = false;
     }
   };
-  // Copies are announced two groups behind, once they have landed.
+  // Copies are announced once they have landed: two groups behind, or all of
+  // them before the thread blocks for a free stage.
   uint64_t* pending[2] = {nullptr, nullptr};
   auto announce = [&](uint64_t* bar) {
     if (bar) {
@@ -171,7 +208,10 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnParams& p, Shared& s, uin
   int tiles = 0;  // ring tiles asked for (16-bit) or filled (8-bit)
   int n_q = 0;    // q loads
   auto load_q = [&](const AttnWalk<Work>& k) {
-    if (n_q > 0) wait(&s.q_empty, (n_q - 1) & 1);
+    if (n_q > 0 && !mbar_test(&s.q_empty, (n_q - 1) & 1)) {
+      flush();
+      wait(&s.q_empty, (n_q - 1) & 1);
+    }
     ++n_q;
     const int rows = k.rows();
     for (int i = 0; i < 2; ++i) {
@@ -215,26 +255,69 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnParams& p, Shared& s, uin
   if constexpr (!FP8) {
     AttnWalk<Work> k(w, share);
     bool more = k.next();
-    if (more) note(0, look_up(k.it, k.u0));
+    // Warp 0's lanes each load one box of whole units.
+    const int boxes = tma.box_rows ? kUnit / tma.box_rows : 0;
+    const int box = lane / kPanels, panel = lane % kPanels;
+    int box_page[2] = {0, 0}, box_row[2] = {0, 0};
+    auto look_up_box = [&](int n, int unit) {
+      if (warp != 0 || box >= boxes) return;
+      const int j = unit * kUnit + box * tma.box_rows;
+      const int pg = j / p.c.page_size;
+      const int page = pg < p.b.max_pages ? p.b.page_table[(long long)k.it.b * p.b.page_table_stride + pg] : 0;
+      const int row = j - pg * p.c.page_size;
+      if (n & 1) {
+        box_page[1] = page;
+        box_row[1] = row;
+      } else {
+        box_page[0] = page;
+        box_row[0] = row;
+      }
+    };
+    auto prepare = [&](int n, int unit) {
+      look_up_box(n, unit);
+      note(n, look_up(k.it, unit));
+    };
+    if (more) prepare(0, k.u0);
     for (int n = 1; more; ++n) {  // the unit whose rows are looked up next
       const int units = k.units;
       for (int j = 0; j < units; ++j, ++n) {
         named_sync(3, 128);  // the unit's rows are known; the one before is done with its
-        for (int kv = 0; kv < 2; ++kv, ++tiles) {
+        const uint32_t* there = s.there[(n - 1) & 7];
+        const bool whole = boxes && (there[0] & there[1] & there[2] & there[3]) == 0xffffffffu;
+        for (int kv = 0; kv < 2; ++kv) {
           const int st = tiles % kStages;
-          if (tiles >= kStages) wait(&s.kv_empty[st], (tiles / kStages - 1) & 1);
-          copy_tile(n - 1, kv == 0 ? p.c.k : p.c.v, smem + kOffRing + st * kTileBytes, false);
-          commit(&s.kv_full[st]);
+          if (tiles >= kStages) {
+            const uint32_t parity = (tiles / kStages - 1) & 1;
+            if (!mbar_test(&s.kv_empty[st], parity)) {
+              flush();
+              wait(&s.kv_empty[st], parity);
+            }
+          }
+          ++tiles;
+          uint64_t* full = &s.kv_full[st];
+          const uint32_t dst = smem + kOffRing + st * kTileBytes;
+          if (whole) {
+            if (tid == 0) mbar_arrive_expect_tx(full, kTileBytes);
+            else mbar_arrive(full);
+            __syncwarp();
+            if (warp == 0 && box < boxes)
+              tma_load_4d(dst + panel * kPanelBytes + box * tma.box_rows * 128, kv == 0 ? &tma.k : &tma.v, panel * 64,
+                          (n & 1) ? box_row[0] : box_row[1], k.it.h, (n & 1) ? box_page[0] : box_page[1], full);
+          } else {
+            copy_tile(n - 1, kv == 0 ? p.c.k : p.c.v, dst, false);
+            commit(full);
+          }
           if (j == 0 && kv == 0) {
             load_q(k);
             commit(&s.q_full);
           }
         }
-        if (j + 1 < units) note(n, look_up(k.it, k.u0 + j + 1));
+        if (whole) flush();  // copies behind which none may come for long
+        if (j + 1 < units) prepare(n, k.u0 + j + 1);
       }
       --n;
       more = k.next();
-      if (more) note(n, look_up(k.it, k.u0));
+      if (more) prepare(n, k.u0);
     }
     flush();
   } else {
@@ -305,74 +388,97 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnParams& p, Shared& s, uin
 // Products
 // ---------------------------------------------------------------------------
 template <typename T, bool FP8, int D>
-__device__ void TilesKernel<T, FP8, D>::multiply(const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share) {
+__device__ void TilesKernel<T, FP8, D>::multiply(const AttnParams& p, Shared& s, uint32_t smem, const AttnShare& share,
+                                       int t) {
   constexpr int kFmt = kBf16 ? 1 : 0;
-  constexpr uint32_t kQk = tc_idesc(1, kFmt, kFmt, 0, kUnit), kPv = tc_idesc(1, kFmt, kFmt, 1, D);
+  constexpr uint32_t kQk = tc_idesc(1, kFmt, kFmt, 0, kStep), kPv = tc_idesc(1, kFmt, kFmt, 1, D);
   const Work w(p);
   AttnWalk<Work> k(w, share);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok && !mbar_wait_bounded(bar, parity)) {
+    if (ok && !mbar_wait_spin(bar, parity)) {
       *p.error = kErrFullWait;
       ok = false;
     }
     tc_fence_after();
   };
   const uint32_t tm = s.tmem;
-  auto wait_tile = [&](int i) { wait(&s.kv_full[i % kStages], (i / kStages) & 1); };
-  auto qk = [&](int t, int i) {  // S_t = Q_t (ring tile i)^T
+  // Places in the ring, kept by counting: this thread's own instructions are
+  // on the way from one product to the next.
+  struct Place {
+    int st = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ Place after() const {
+      Place r;
+      r.st = st + 1 == kStages ? 0 : st + 1;
+      r.parity = parity ^ (st + 1 == kStages);
+      return r;
+    }
+  };
+  const uint64_t q_desc = smem_desc_sw128(smem, 16, 1024), k_desc = smem_desc_sw128(smem + kOffRing, 16, 1024),
+                 v_desc = smem_desc_sw128(smem + kOffRing, kPanelBytes, 1024);
+  auto qk = [&](const Place& at, int half) {  // S_t[half] = Q_t (half of K)^T
     if (!ok) return;
-    const uint64_t a = smem_desc_sw128(smem + t * kTileBytes, 16, 1024);
-    const uint64_t b = smem_desc_sw128(smem + kOffRing + (i % kStages) * kTileBytes, 16, 1024);
+    const uint64_t a = q_desc + t * (kTileBytes >> 4), b = k_desc + at.st * (kTileBytes >> 4) + half * (kStep * 128 >> 4);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
       const uint32_t off = ((ks >> 2) * kPanelBytes + (ks & 3) * 32) >> 4;
-      mma_f16_ss(tm + t * kUnit, a + off, b + off, kQk, ks > 0);
+      mma_f16_ss(tm + t * kUnit + half * kStep, a + off, b + off, kQk, ks > 0);
     }
   };
-  auto pv = [&](int t, int i, bool first) {  // O_t (+)= P_t (ring tile i)
+  auto pv = [&](const Place& at, int half, bool first) {  // O_t (+)= P_t[half] (half of V)
     if (!ok) return;
-    const uint64_t b = smem_desc_sw128(smem + kOffRing + (i % kStages) * kTileBytes, kPanelBytes, 1024);
+    const uint64_t b = v_desc + at.st * (kTileBytes >> 4) + half * (kStep * 128 >> 4);
 #pragma unroll
-    for (int ks = 0; ks < kUnit / 16; ++ks)
-      mma_f16_ts(tm + 2 * kUnit + t * D, tm + t * kUnit + ks * 8, b + ((ks * 2048) >> 4), kPv, !first || ks > 0);
+    for (int ks = 0; ks < kStep / 16; ++ks)
+      mma_f16_ts(tm + 2 * kUnit + t * D, tm + t * kUnit + half * kStep + ks * 8, b + ((ks * 2048) >> 4), kPv,
+                 !first || ks > 0);
   };
-  int i = 0, segs = 0;        // ring tiles so far, segments
-  uint32_t p_par[2] = {0, 0};
+  Place kp;  // of the next keys
+  uint32_t q_par = 0, p_par = 0;
   while (k.next()) {
-    const int nt = k.rows() > kTile ? 2 : 1;
-    wait(&s.q_full, segs & 1);
-    wait_tile(i);
-    for (int t = 0; t < nt; ++t) {
-      qk(t, i);
-      tc_commit(&s.s_full[t]);
-    }
-    tc_commit(&s.kv_empty[i % kStages]);
-    if (k.units == 1) tc_commit(&s.q_empty);
-    for (int j = 0; j < k.units; ++j, i += 2) {
-      const bool last = j + 1 == k.units;
-      wait_tile(i + 1);
-      for (int t = 0; t < nt; ++t) {
-        wait(&s.p_full[t], p_par[t]);
-        p_par[t] ^= 1;
-        pv(t, i + 1, j == 0);
-        if (last) {
-          tc_commit(&s.o_full[t]);
-        } else {
-          if (t == 0) wait_tile(i + 2);
-          qk(t, i + 2);
-          tc_commit(&s.s_full[t]);
-        }
+    const bool mine = t * kTile < k.rows();  // else this warp only hands the stages back
+    const int units = k.units;
+    auto give_back = [&](uint64_t* bar) {
+      if (mine) tc_commit(bar);
+      else mbar_arrive(bar);
+    };
+    wait(&s.q_full, q_par);
+    q_par ^= 1;
+    wait(&s.kv_full[kp.st], kp.parity);
+    if (mine) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        qk(kp, half);
+        tc_commit(&s.s_full[t][half]);
       }
-      tc_commit(&s.kv_empty[(i + 1) % kStages]);
-      if (!last) tc_commit(&s.kv_empty[(i + 2) % kStages]);
-      if (j + 2 == k.units) tc_commit(&s.q_empty);
     }
-    ++segs;
+    give_back(&s.kv_empty[kp.st]);
+    if (units == 1) give_back(&s.q_empty);
+    for (int j = 0; j < units; ++j) {
+      const bool last = j + 1 == units;
+      const Place vp = kp.after();
+      kp = vp.after();
+      wait(&s.kv_full[vp.st], vp.parity);
+      if (!last) wait(&s.kv_full[kp.st], kp.parity);
+      if (mine) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          wait(&s.p_full[t][half], p_par);
+          pv(vp, half, j == 0 && half == 0);
+          if (!last) qk(kp, half);
+          tc_commit(&s.s_full[t][half]);  // the next scores, or (the last time) O
+        }
+        p_par ^= 1;
+      }
+      give_back(&s.kv_empty[vp.st]);
+      if (!last) give_back(&s.kv_empty[kp.st]);
+      if (j + 2 == units) give_back(&s.q_empty);
+    }
   }
   if (!ok) {
-    tc_commit(&s.drain);
-    mbar_wait_bounded(&s.drain, 0);
+    tc_commit(&s.drain[t]);
+    mbar_wait_spin(&s.drain[t], 0);
   }
 }
 
@@ -388,14 +494,14 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
   AttnWalk<Work> k(w, share);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok && !mbar_wait_bounded(bar, parity)) {
+    if (ok && !mbar_wait_spin(bar, parity)) {
       *p.error = kErrFullWait;
       ok = false;
     }
     __syncwarp();
     tc_fence_after();
   };
-  uint32_t s_par = 0, o_par = 0;
+  uint32_t s_par[2] = {0, 0};
   int n = 0;  // units of this block so far
   while (k.next()) {
     const int rows = k.rows();
@@ -414,24 +520,26 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
         p.a.window > 0 ? k.it.s.ctx + (k.it.tile * kRows + min(tile * kTile + kTile, rows) - 1) / p.group - p.a.window : -1;
     float scale = p.a.scale * kLog2e * (FP8 && p.c.k_scale ? p.c.k_scale[k.it.h] : 1.0f);
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < k.units; ++j, ++n) {
-      const int j0 = (k.u0 + j) * kUnit;
-      wait(&s.s_full[tile], s_par);
-      s_par ^= 1;
+    for (int u = 0; u < 2 * k.units; ++u) {
+      const int half = u & 1;
+      const int j0 = k.u0 * kUnit + u * kStep;
+      const uint32_t at = tm_s + half * kStep;
+      wait(&s.s_full[tile][half], s_par[half]);
+      s_par[half] ^= 1;
+      uint32_t x[2][32];
+      tmem_ld32(at, x[0]);
+      tmem_ld32(at + 32, x[1]);
       if constexpr (kScaleQ) {
-        if (j == 0) scale *= 1.0f / __uint_as_float((uint32_t)s.q_exp[r] << 23);
+        if (u == 0) scale *= 1.0f / __uint_as_float((uint32_t)s.q_exp[r] << 23);
       }
-      uint32_t x[4][32];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, x[i]);
-      const uint32_t* there = s.there[n & 7];
-      const uint32_t all = there[0] & there[1] & there[2] & there[3];
+      const uint2 there = *reinterpret_cast<const uint2*>(&s.there[(n + (u >> 1)) & 7][2 * half]);
+      const bool masked = (there.x & there.y) != 0xffffffffu || j0 + kStep - 1 > first_pos || j0 <= last_low;
       tmem_wait_ld();
-      if (all != 0xffffffffu || j0 + kUnit - 1 > first_pos || j0 <= last_low) {
+      if (__builtin_expect(masked, 0)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           const int below = row_pos - (j0 + 32 * i) + 1, hidden = low - (j0 + 32 * i) + 1;
-          uint32_t mask = there[i];
+          uint32_t mask = i ? there.y : there.x;
           mask &= below >= 32 ? 0xffffffffu : below <= 0 ? 0u : (1u << below) - 1;
           mask &= hidden >= 32 ? 0u : hidden <= 0 ? 0xffffffffu : ~((1u << hidden) - 1);
 #pragma unroll
@@ -439,55 +547,58 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
             if (!(mask >> c & 1)) x[i][c] = 0xff800000u;
         }
       }
-      float mx[4];
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mx[i] = __uint_as_float(x[i][0]);
-#pragma unroll
-        for (int c = 1; c < 32; ++c) mx[i] = fmaxf(mx[i], __uint_as_float(x[i][c]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-      if (j == 0) {
+      for (int c = 0; c < 64; c += 2)
+        mx[c / 2 % 4] = max3(mx[c / 2 % 4], __uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1]));
+      const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
+      if (u == 0) {
         m = top;
       } else {
-        const bool grown = top > m + 8.0f;
-        if (__any_sync(0xffffffffu, grown)) {
+        const bool grown = !(top <= m + 8.0f);  // also where top is NaN: the row becomes NaN
+        if (__builtin_expect(__any_sync(0xffffffffu, grown), 0)) {
           const float by = grown ? exp2_fast(m - top) : 1.0f;
           if (grown) m = top;
           l *= by;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t o[32];
-            tmem_ld32(tm_o + 32 * i, o);
+          // The other buffer's next phase comes behind the last step's products.
+          wait(&s.s_full[tile][half ^ 1], s_par[half ^ 1]);
+#pragma unroll 1
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t o[16];
+            tmem_ld16(tm_o + 16 * i, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * by);
-            tmem_st32(tm_o + 32 * i, o);
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * by);
+            tmem_st16(tm_o + 16 * i, o);
           }
         }
       }
       const float neg = m == -INFINITY ? 0.f : -m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = pair2(scale, scale), neg2 = pair2(neg, neg);
+      uint64_t sum[2] = {0, 0};
+      uint32_t pk[32];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float a = exp2_fast(fmaf(__uint_as_float(x[2 * i + c / 32][c % 32]), scale, neg));
-          const float b = exp2_fast(fmaf(__uint_as_float(x[2 * i + c / 32][c % 32 + 1]), scale, neg));
-          sum[c & 2] += a;
-          sum[(c & 2) + 1] += b;
-          pk[c / 2] = Act<P16>::pack(a, b);
-        }
-        tmem_st32(tm_s + 32 * i, pk);
+      for (int c = 0; c < 64; c += 2) {
+        const uint64_t t2 =
+            fma2(pair2(__uint_as_float(x[c / 32][c % 32]), __uint_as_float(x[c / 32][c % 32 + 1])), scale2, neg2);
+        const float2 t = unpair2(t2);
+        const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+        sum[c / 2 & 1] = add2(sum[c / 2 & 1], pair2(e.x, e.y));
+        pk[c / 2] = Act<P16>::pack(e.x, e.y);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st32(at, pk);
+      const float2 both = unpair2(add2(sum[0], sum[1]));
+      l += both.x + both.y;
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&s.p_full[tile]);
+      mbar_arrive(&s.p_full[tile][half]);
     }
-    wait(&s.o_full[tile], o_par);
-    o_par ^= 1;
+    n += k.units;
+    // Each buffer's last phase: O is complete.
+    wait(&s.s_full[tile][0], s_par[0]);
+    wait(&s.s_full[tile][1], s_par[1]);
+    s_par[0] ^= 1;
+    s_par[1] ^= 1;
 
     const float vs = FP8 && p.c.v_scale ? p.c.v_scale[k.it.h] : 1.0f;
     const long long t = k.it.s.first + tok;
@@ -501,10 +612,11 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
                        Act<T>::pack(v[c + 4] * inv, v[c + 5] * inv), Act<T>::pack(v[c + 6] * inv, v[c + 7] * inv));
     };
     auto write_lse = [&](float mm, float ll) {
-      if (p.a.lse) p.a.lse[t * p.q_heads + h] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) / kLog2e;
+      if (p.a.lse) p.a.lse[t * p.q_heads + h] = mm == -INFINITY ? -INFINITY : (mm + log2f(ll)) / kLog2e;
     };
     if (!k.split()) {
-      const float inv = l == 0.f ? 0.f : vs / l;
+      const bool none = m == -INFINITY;  // nothing seen
+      const float inv = none ? 0.f : vs / l;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         uint32_t o[32];
@@ -512,7 +624,7 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
         tmem_wait_ld();
         float f[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) f[c] = l == 0.f ? 0.f : __uint_as_float(o[c]);
+        for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(o[c]);
         if (in) write32(32 * i, f, inv);
       }
       if (in) write_lse(m, l);
@@ -555,7 +667,7 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
 #pragma unroll 4
         for (int c = c_first; c <= c_last; ++c)
           ll += __ldcg(part(c) + kTile * D + kTile + tid) * exp2_fast(__ldcg(part(c) + kTile * D + tid) - base);
-        const float inv = ll == 0.f ? 0.f : vs / ll;
+        const float inv = mm == -INFINITY ? 0.f : vs / ll;
         for (int i = 0; i < D / 32; ++i) {
           float f[32] = {};
 #pragma unroll 2
@@ -580,7 +692,8 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
 }
 
 template <typename T, bool FP8, int D>
-__global__ void __launch_bounds__(512, 1) attn_tiles_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(512, 1) attn_tiles_kernel(const __grid_constant__ AttnTilesParams a) {
+  const AttnParams& p = a.p;
   using K = TilesKernel<T, FP8, D>;
   extern __shared__ __align__(1024) uint8_t dyn[];
   __shared__ typename K::Shared s;
@@ -593,16 +706,16 @@ __global__ void __launch_bounds__(512, 1) attn_tiles_kernel(const __grid_constan
   if (threadIdx.x == 0) {
     for (int i = 0; i < K::kStages; ++i) {
       mbar_init(&s.kv_full[i], 128);
-      mbar_init(&s.kv_empty[i], 1);
+      mbar_init(&s.kv_empty[i], 2);
     }
     mbar_init(&s.q_full, 128);
-    mbar_init(&s.q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], 128);
-      mbar_init(&s.o_full[i], 1);
+    mbar_init(&s.q_empty, 2);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s.s_full[i >> 1][i & 1], 1);
+      mbar_init(&s.p_full[i >> 1][i & 1], 128);
     }
-    mbar_init(&s.drain, 1);
+    mbar_init(&s.drain[0], 1);
+    mbar_init(&s.drain[1], 1);
     fence_mbarrier_init();
   }
   if (warp == 12) tmem_alloc(&s.tmem, 512);
@@ -612,16 +725,12 @@ __global__ void __launch_bounds__(512, 1) attn_tiles_kernel(const __grid_constan
   const typename K::Work w(p);
   const AttnShare share = attn_share(w, p.least_units, s.share);  // synchronises the block
   tc_fence_after();
-  // 512 threads of 128 registers: 2 x 128 x 192 + 2 x 128 x 64 is the same sum.
   if (warp < 8) {
-    reg_inc<192>();
     K::softmax(p, s, share, warp >> 2);
   } else if (warp < 12) {
-    reg_dec<64>();
-    K::load(p, s, smem, share);
+    K::load(a.tma, p, s, smem, share);
   } else {
-    reg_dec<64>();
-    if (threadIdx.x == 12 * 32) K::multiply(p, s, smem, share);
+    if (warp < 14 && (threadIdx.x & 31) == 0) K::multiply(p, s, smem, share, warp - 12);
   }
   __syncwarp();
   tc_fence_before();

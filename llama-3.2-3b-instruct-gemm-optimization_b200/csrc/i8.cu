@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         for (int k = s.k0; k < s.k1; ++k, ++i) {
           const int stage = i % t.stages;
           if (i >= issued) {
-            if (i >= t.stages && !mbar_wait_bounded(&empty[stage], (i / t.stages - 1) & 1)) {
+            if (i >= t.stages && !mbar_wait_spin(&empty[stage], (i / t.stages - 1) & 1)) {
               *t.error = kErrEmptyWait;
               ok = false;
               break;
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         }
       // After an error the copies in flight land before this CTA's memory goes.
       if (!ok)
-        for (int j = max(0, i - t.stages); j < i; ++j) mbar_wait_bounded(&full[j % t.stages], (j / t.stages) & 1);
+        for (int j = max(0, i - t.stages); j < i; ++j) mbar_wait_spin(&full[j % t.stages], (j / t.stages) & 1);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
       bool ok = true;
       while (ok && s.next(t)) {
         const int buf = n & 1;
-        if (!mbar_wait_bounded(&acc_empty[buf], ((n >> 1) & 1) ^ 1)) {
+        if (!mbar_wait_spin(&acc_empty[buf], ((n >> 1) & 1) ^ 1)) {
           *t.error = kErrEmptyWait;
           ok = false;
           break;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         tc_fence_after();
         for (int k = s.k0; k < s.k1; ++k, ++i) {
           const int stage = i % t.stages;
-          if (!mbar_wait_bounded(&full[stage], (i / t.stages) & 1)) {
+          if (!mbar_wait_spin(&full[stage], (i / t.stages) & 1)) {
             *t.error = kErrFullWait;
             ok = false;
             break;
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
       }
       if (!ok) {
         tc_commit(&drain);
-        mbar_wait_bounded(&drain, 0);
+        mbar_wait_spin(&drain, 0);
       }
     }
   } else {
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
       };
       if (t.cluster == 1) load_residual(0);
       named_sync(1, 128);
-      if (!mbar_wait_bounded(&acc_full[buf], (n >> 1) & 1)) {
+      if (!mbar_wait_spin(&acc_full[buf], (n >> 1) & 1)) {
         *t.error = kErrFullWait;
         break;
       }
@@ -573,22 +573,6 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, t.tmem_cols);
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point.
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  return fn;
 }
 
 // Rows of bytes, 128 columns by box_rows a load, zeros outside.

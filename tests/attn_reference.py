@@ -42,7 +42,7 @@ def attention(q, k_cache, v_cache, new, total, table, layout="NHD", k_scale=None
     that holds the probabilities and r that of out:
       probabilities rounded once:  u A, and at most 2^-25 each below fp16's
                                    normal range (the largest is 1): 2^-25 sum |v| / l
-      a score's error e (dot of n products in fp32, scale, 2^x to 2^-22) moves
+      a score's error e (dot of n products in fp32, scale, 2^x to 2^-18) moves
       a weight by at most 2 e:     2 e A
       sums of weights and of products over the tokens in fp32: tokens 2^-24 A
       the result rounded:          r |out|
@@ -83,7 +83,7 @@ def attention(q, k_cache, v_cache, new, total, table, layout="NHD", k_scale=None
             o = w @ vv
             out[own, h] = o
             mag = (qq.abs() @ kk.abs().T * scale).masked_fill(~sees, 0).amax(1, keepdim=True)
-            e = (d + 4) * 2.0 ** -24 * mag + 2.0 ** -21
+            e = (d + 4) * 2.0 ** -24 * mag + 2.0 ** -18
             a = w @ vv.abs()
             ell = torch.exp(lse[own, h] - s.amax(1))[:, None].nan_to_num(1.0).clamp(min=1.0)
             small = 2.0 ** -25 * (sees.double() @ vv.abs()) / ell if u < 2.0 ** -9 else 0
