@@ -424,7 +424,7 @@ b2g_status b2g_i8_quantize_rows(const b2g_i8_rows_args* args, b2g_stream_t strea
 b2g_status b2g_i8_quantize_weights(const void* w16, int32_t K, int32_t N, int32_t layout, int32_t dtype,
                                    void* codes, int64_t ld_codes, float* scales, b2g_stream_t stream);
 
-#define B2G_I8_MAX_K 131072 /* the int32 sum of this many products cannot overflow */
+#define B2G_I8_MAX_K 131071 /* the int32 sum of this many products (128 * 128 at most) cannot overflow */
 typedef struct {
   int32_t in_features;  /* K, 1..B2G_I8_MAX_K */
   int32_t out_features; /* N (per weight plane) */

@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
   }
   __syncthreads();
   if (ty == 0) {
+    a = 0.f;
     for (int i = 0; i < 32; ++i) a = max_abs(a, tile[i][tx]);
     const float s = scale_of(a);
     inv[tx] = s == s ? 1.0f / s : 0.f;
