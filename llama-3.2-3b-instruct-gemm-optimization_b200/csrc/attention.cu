@@ -15,8 +15,7 @@ cudaError_t launch_rows(AttnParams p, int num_sms, cudaStream_t stream) {
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, FP8, D>), K::kSmem, &allowed);
   if (e != cudaSuccess) return e;
   p.least_units = 4;
-  // Two blocks an SM, or what the longest possible work fills.
-  return launch_after(attn_rows_kernel<T, FP8, D>, dim3(2 * num_sms), dim3(128), K::kSmem, 1, stream, p);
+  return launch_after(attn_rows_kernel<T, FP8, D>, dim3(K::kBlocks * num_sms), dim3(128), K::kSmem, 1, stream, p);
 }
 
 // A 16-bit cache as (dim, row, head, page); loads of 64 elements by `rows`.
@@ -71,9 +70,9 @@ cudaError_t launch_typed(const AttnParams& p, int num_sms, cudaStream_t stream) 
 
 }  // namespace
 
-size_t attn_counter_bytes(int num_sms) { return ((size_t)num_sms * 2 * 4 + 255) / 256 * 256; }
+size_t attn_counter_bytes(int num_sms) { return ((size_t)num_sms * 3 * 4 + 255) / 256 * 256; }
 size_t attn_part_bytes(int num_sms, int head_dim) {
-  const size_t rows = 2 * (size_t)(head_dim * 16 + 32), tiles = 2 * (size_t)(head_dim * 128 + 256);
+  const size_t rows = 3 * (size_t)(head_dim * 16 + 32), tiles = 2 * (size_t)(head_dim * 128 + 256);
   static_assert(RowsKernel<__half, false, 64>::kPartFloats == 64 * 16 + 32 &&
                     TilesKernel<__half, false, 64>::kPartFloats == 64 * 128 + 256,
                 "a block's parts");

@@ -68,10 +68,11 @@ struct RowsKernel {
   static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
   static constexpr int kTileBytes = 16 * kRowBytes;       // 16 tokens of keys or values
   static constexpr int kStageBytes = 2 * kTileBytes;      // of one warp
-  static constexpr int kStages = 24576 / kStageBytes;     // 24 KB a warp in flight
+  static constexpr int kBlocks = FP8 ? 2 : 2;        // an SM
+  static constexpr int kStages = 49152 / kBlocks / kStageBytes;  // 48 KB of a warp's place in flight
   static constexpr int kNT = D / 8;                       // output tiles of 8 columns
   static constexpr int kSmem = kWarps * kStages * kStageBytes + kNT * 32 * 16;
-  static constexpr int kPartFloats = kNT * 32 * 4 + 32;   // a part: fragments, then maximum and sum of 16 rows
+  static constexpr int kPartFloats = 16 * D + 32;         // a part: [row][column], then maxima and sums of 16 rows
 
   using Work = AttnWork<kRows, kUnit>;
 
@@ -96,7 +97,7 @@ template <typename T, bool FP8, int D>
 __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ long long sh[8];
-  __shared__ float sh_ml[2][16];
+  __shared__ float sh_ml[2][16], sh_red[8][16];
   __shared__ int sh_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   const uint32_t ring = smem_addr(smem) + warp * kStages * kStageBytes;
@@ -248,7 +249,8 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
       const uint32_t kt = ring + stage * kStageBytes, vt = kt + kTileBytes;
       stage = stage == kStages - 1 ? 0 : stage + 1;
       if (here != 0) {
-        float s[2][4] = {};
+        // Even and odd k steps in sums of their own: chains of half the length.
+        float s[2][4] = {}, s_odd[2][4] = {};
         if constexpr (!FP8) {
           // Matrices: tokens 0-7 / 8-15 by d halves of a k16 step.
           const int t = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
@@ -256,25 +258,25 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
           for (int ss = 0; ss < D / 16; ++ss) {
             uint32_t b[4];
             ldsm4(b, kt + chunk_at(t, 2 * ss + half));
-            mma_act<kBf16>(s[0], qf[ss], b[0], b[1]);
-            mma_act<kBf16>(s[1], qf[ss], b[2], b[3]);
+            mma_act<kBf16>(ss & 1 ? s_odd[0] : s[0], qf[ss], b[0], b[1]);
+            mma_act<kBf16>(ss & 1 ? s_odd[1] : s[1], qf[ss], b[2], b[3]);
           }
         } else {
           // A product over d may take d in any order: lane quarter q takes the
           // 16 bytes q (and 4 + q) of a token, four k16 steps of 2 + 2.
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
+          for (int hf = 0; hf < D / 64; ++hf) {
+            const uint4 v0 = lds128_at(kt + chunk_at(g, hf * 4 + q4)), v1 = lds128_at(kt + chunk_at(8 + g, hf * 4 + q4));
+            const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-            for (int hf = 0; hf < D / 64; ++hf) {
-              const uint4 v = lds128_at(kt + chunk_at(nt * 8 + g, hf * 4 + q4));
-              const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t b0, b1;
-                e4m3x4_to_f16x2x2(wd[i], b0, b1);
-                mma_act<false>(s[nt], qf[hf * 4 + i], b0, b1);
-              }
+            for (int i = 0; i < 4; ++i) {
+              uint32_t b0, b1;
+              e4m3x4_to_f16x2x2(w0[i], b0, b1);
+              mma_act<false>(i & 1 ? s_odd[0] : s[0], qf[hf * 4 + i], b0, b1);
+              e4m3x4_to_f16x2x2(w1[i], b0, b1);
+              mma_act<false>(i & 1 ? s_odd[1] : s[1], qf[hf * 4 + i], b0, b1);
             }
+          }
         }
         // Scores of rows g, g + 8 and tokens 8 nt + 2q, + 1.
         const int j0 = (u0 + n) * kUnit + warp * 16;
@@ -285,7 +287,7 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
           for (int e = 0; e < 4; ++e) {
             const int t = nt * 8 + 2 * q4 + (e & 1), j = j0 + t, hf = e >> 1;
             const bool sees = j <= row_pos[hf] && j > low[hf] && (here >> t & 1);
-            s[nt][e] = sees ? s[nt][e] * scale[hf] : -INFINITY;
+            s[nt][e] = sees ? (s[nt][e] + s_odd[nt][e]) * scale[hf] : -INFINITY;
             mx[hf] = fmaxf(mx[hf], s[nt][e]);
           }
         float al[2];
@@ -390,49 +392,72 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
       __syncthreads();
     }
     const float vs = FP8 && p.c.v_scale ? p.c.v_scale[it.h] : 1.0f;
-    auto write = [&](int hf, float mm, float ll, auto value, int j_from, int j_to) {
-      const int r = it.tile * kRows + g + 8 * hf;
-      if (r >= rows) return;
-      const int i = r / p.group, h = it.h * p.group + r - i * p.group;
-      const long long t = it.s.first + i;
-      const float inv = ll == 0.f ? 0.f : vs / ll;
-      T* out = static_cast<T*>(p.a.out) + t * p.a.stride_o + h * p.a.stride_o_head;
+    const int valid = min(rows - it.tile * kRows, kRows);  // rows of the tile
+    // Two (or, 8-bit: four, tiles j and j + 1 interleave) consecutive columns
+    // of row g + 8 hf at a time.
+    auto pieces = [&](int hf, auto take) {
 #pragma unroll
-      for (int j = 0; j < kNT; ++j) {
-        if (j < j_from || j >= j_to) continue;
-        if constexpr (FP8) {
-          if (j & 1) continue;  // tiles j, j + 1 interleave: four consecutive columns
-          uint2 v;
-          v.x = Act<T>::pack(value(j, 2 * hf) * inv, value(j + 1, 2 * hf) * inv);
-          v.y = Act<T>::pack(value(j, 2 * hf + 1) * inv, value(j + 1, 2 * hf + 1) * inv);
-          *reinterpret_cast<uint2*>(out + column(j, q4, 0)) = v;
-        } else {
-          *reinterpret_cast<uint32_t*>(out + column(j, q4, 0)) =
-              Act<T>::pack(value(j, 2 * hf) * inv, value(j, 2 * hf + 1) * inv);
-        }
+      for (int j = 0; j < kNT; j += FP8 ? 2 : 1) {
+        if constexpr (FP8)
+          take(column(j, q4, 0), o[j][2 * hf], o[j + 1][2 * hf], o[j][2 * hf + 1], o[j + 1][2 * hf + 1]);
+        else
+          take(column(j, q4, 0), o[j][2 * hf], o[j][2 * hf + 1], 0.f, 0.f);
       }
-      if (p.a.lse && q4 == 0 && j_from == 0)
-        p.a.lse[t * p.q_heads + h] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) / kLog2e;
+    };
+    auto place = [&](int r, long long* t, int* h) {  // token and head of row r of the tile
+      const int rr = it.tile * kRows + r, i = rr / p.group;
+      *t = it.s.first + i;
+      *h = it.h * p.group + rr - i * p.group;
+    };
+    auto write_lse = [&](long long t, int h, float mm, float ll) {
+      if (p.a.lse) p.a.lse[t * p.q_heads + h] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) / kLog2e;
     };
     if (!split) {
-      if (warp == 0)
-        for (int hf = 0; hf < 2; ++hf) write(hf, m[hf], l[hf], [&](int j, int e) { return o[j][e]; }, 0, kNT);
+      if (warp == 0) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int r = g + 8 * hf;
+          if (r >= valid) continue;
+          long long t;
+          int h;
+          place(r, &t, &h);
+          const float inv = l[hf] == 0.f ? 0.f : vs / l[hf];
+          T* out = static_cast<T*>(p.a.out) + t * p.a.stride_o + h * p.a.stride_o_head;
+          pieces(hf, [&](int col, float a, float b, float c, float d) {
+            if constexpr (FP8)
+              *reinterpret_cast<uint2*>(out + col) =
+                  make_uint2(Act<T>::pack(a * inv, b * inv), Act<T>::pack(c * inv, d * inv));
+            else
+              *reinterpret_cast<uint32_t*>(out + col) = Act<T>::pack(a * inv, b * inv);
+          });
+          if (q4 == 0) write_lse(t, h, m[hf], l[hf]);
+        }
+      }
     } else {
       // This block's part, and the join by the last block to arrive.
       float* parts = static_cast<float*>(p.parts);
       const int c_first = attn_owner(share, item_begin);
       const int c_last = attn_owner(share, item_begin + (it.u_hi - it.u_lo) - 1);
+      // A block's first segment is its part 0; only the item's first block can
+      // have begun before it.
+      const int first_part = attn_begin(share, c_first) < item_begin;
+      auto part = [&](int c) { return parts + (c * 2 + (c == c_first ? first_part : 0)) * (long long)kPartFloats; };
       if (warp == 0) {
-        float* mine = parts + ((long long)blockIdx.x * 2 + (pos - units != share.begin)) * kPartFloats;
-        float4* po = reinterpret_cast<float4*>(mine);
+        float* mine = part(blockIdx.x);
 #pragma unroll
-        for (int j = 0; j < kNT; ++j) __stcg(po + j * 32 + lane, make_float4(o[j][0], o[j][1], o[j][2], o[j][3]));
-        if (q4 == 0) {
-          float* ml = mine + kNT * 32 * 4;
-          __stcg(ml + g, m[0]);
-          __stcg(ml + g + 8, m[1]);
-          __stcg(ml + 16 + g, l[0]);
-          __stcg(ml + 24 + g, l[1]);
+        for (int hf = 0; hf < 2; ++hf) {
+          const int r = g + 8 * hf;
+          if (r >= valid) continue;
+          pieces(hf, [&](int col, float a, float b, float c, float d) {
+            if constexpr (FP8)
+              __stcg(reinterpret_cast<float4*>(mine + r * D + col), make_float4(a, b, c, d));
+            else
+              __stcg(reinterpret_cast<float2*>(mine + r * D + col), make_float2(a, b));
+          });
+          if (q4 == 0) {
+            __stcg(mine + 16 * D + r, m[hf]);
+            __stcg(mine + 16 * D + 16 + r, l[hf]);
+          }
         }
         __threadfence();
         __syncwarp();
@@ -445,48 +470,93 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
       __syncthreads();
       if (sh_last) {
         __threadfence();
-        auto part = [&](int c) {
-          const bool first = (long long)c * share.total / share.blocks >= item_begin;
-          return parts + ((long long)c * 2 + (first ? 0 : 1)) * kPartFloats;
-        };
-        // Every warp joins a quarter of the columns, in the blocks' order.
-        constexpr int NJ = kNT / kWarps;
-        const bool low_only = rows - it.tile * kRows <= 8;
-        float mm[2] = {-INFINITY, -INFINITY};
-#pragma unroll 4
-        for (int c = c_first; c <= c_last; ++c) {
-          const float* ml = part(c) + kNT * 32 * 4;
-          mm[0] = fmaxf(mm[0], __ldcg(ml + g));
-          mm[1] = fmaxf(mm[1], __ldcg(ml + g + 8));
-        }
-        const float base[2] = {mm[0] == -INFINITY ? 0.f : mm[0], mm[1] == -INFINITY ? 0.f : mm[1]};
-        float ll[2] = {0.f, 0.f}, acc[NJ][4] = {};
-#pragma unroll 4
-        for (int c = c_first; c <= c_last; ++c) {
-          const float* ml = part(c) + kNT * 32 * 4;
-          const float a0 = exp2_fast(__ldcg(ml + g) - base[0]), a1 = exp2_fast(__ldcg(ml + g + 8) - base[1]);
-          ll[0] += __ldcg(ml + 16 + g) * a0;
-          ll[1] += __ldcg(ml + 24 + g) * a1;
-          const float4* po = reinterpret_cast<const float4*>(part(c)) + warp * NJ * 32 + lane;
+        // The parts' weights, 32 parts at a time, in the join buffer: [part][row].
+        constexpr int kChunk = 32;
+        static_assert(kChunk * 16 * 4 <= kNT * 32 * 16, "join buffer");
+        const int r = threadIdx.x & 15, lead = threadIdx.x >> 4;  // eight parts at once
+        // The first chunk's maxima and sums are kept; more than 32 parts are rare.
+        float mc[kChunk / 8], lc[kChunk / 8], mm = -INFINITY;
+        auto load_ml = [&](int c0) {
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            const float4 v = __ldcg(po + j * 32);
-            acc[j][0] += v.x * a0;
-            acc[j][1] += v.y * a0;
-            acc[j][2] += v.z * a1;
-            acc[j][3] += v.w * a1;
+          for (int i = 0; i < kChunk / 8; ++i) {
+            const int c = c0 + lead + 8 * i;
+            mc[i] = -INFINITY;
+            lc[i] = 0.f;
+            if (c > c_last || r >= valid) continue;
+            mc[i] = __ldcg(part(c) + 16 * D + r);
+            lc[i] = __ldcg(part(c) + 16 * D + 16 + r);
+          }
+        };
+        for (int c = c_first + kChunk + lead; c <= c_last; c += 8)
+          if (r < valid) mm = fmaxf(mm, __ldcg(part(c) + 16 * D + r));
+        load_ml(c_first);
+#pragma unroll
+        for (int i = 0; i < kChunk / 8; ++i) mm = fmaxf(mm, mc[i]);
+        sh_red[lead][r] = mm;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mm = fmaxf(mm, sh_red[i][r]);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        constexpr int kVec = D / 4, kMine = 16 * kVec / 128;  // four columns a thread, kMine times
+        float4 acc[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ll = 0.f;
+        for (int c0 = c_first; c0 <= c_last; c0 += kChunk) {
+          const int n = min(kChunk, c_last + 1 - c0);
+          if (c0 > c_first) load_ml(c0);
+#pragma unroll
+          for (int i = 0; i < kChunk / 8; ++i) {
+            const float a = exp2_fast(mc[i] - base);
+            ll += lc[i] * a;
+            join[(lead + 8 * i) * 16 + r] = a;
+          }
+          __syncthreads();
+#pragma unroll 8
+          for (int c = 0; c < n; ++c) {
+            const float4* po = reinterpret_cast<const float4*>(part(c0 + c));
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              const int at = threadIdx.x + 128 * i, row = at / kVec;
+              if (row >= valid) continue;
+              const float a = join[c * 16 + row];
+              const float4 v = __ldcg(po + at);
+              acc[i].x += v.x * a;
+              acc[i].y += v.y * a;
+              acc[i].z += v.z * a;
+              acc[i].w += v.w * a;
+            }
+          }
+          __syncthreads();
+        }
+        __syncthreads();
+        sh_red[lead][r] = ll;
+        __syncthreads();
+        if (lead == 0) {
+          ll = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ll += sh_red[i][r];
+          sh_ml[0][r] = ll;
+          if (r < valid) {
+            long long t;
+            int h;
+            place(r, &t, &h);
+            write_lse(t, h, mm, ll);
           }
         }
-        for (int hf = 0; hf < (low_only ? 1 : 2); ++hf)
-          write(hf, mm[hf], ll[hf],
-                [&](int j, int e) {
-                  float v = 0.f;
+        __syncthreads();
 #pragma unroll
-                  for (int i = 0; i < NJ; ++i)
-                    if (j == warp * NJ + i) v = acc[i][e];
-                  return v;
-                },
-                warp * NJ, (warp + 1) * NJ);
+        for (int i = 0; i < kMine; ++i) {
+          const int at = threadIdx.x + 128 * i, row = at / kVec;
+          if (row >= valid) continue;
+          long long t;
+          int h;
+          place(row, &t, &h);
+          const float inv = sh_ml[0][row] == 0.f ? 0.f : vs / sh_ml[0][row];
+          T* out = static_cast<T*>(p.a.out) + t * p.a.stride_o + h * p.a.stride_o_head + (at - row * kVec) * 4;
+          *reinterpret_cast<uint2*>(out) = make_uint2(Act<T>::pack(acc[i].x * inv, acc[i].y * inv),
+                                                      Act<T>::pack(acc[i].z * inv, acc[i].w * inv));
+        }
       }
       __syncthreads();
     }
@@ -498,7 +568,7 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
 }
 
 template <typename T, bool FP8, int D>
-__global__ void __launch_bounds__(128, 2) attn_rows_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(128, RowsKernel<T, FP8, D>::kBlocks) attn_rows_kernel(const __grid_constant__ AttnParams p) {
   RowsKernel<T, FP8, D>::run(p);
 }
 

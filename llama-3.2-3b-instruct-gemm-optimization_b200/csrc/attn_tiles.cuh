@@ -632,9 +632,11 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
       float* parts = static_cast<float*>(p.parts);
       const int c_first = attn_owner(share, k.origin);
       const int c_last = attn_owner(share, k.origin + (k.it.u_hi - k.it.u_lo) - 1);
-      auto part = [&](int c) {  // its first segment unless it began before this item
-        const bool first = (long long)c * share.total / share.blocks >= k.origin;
-        return parts + (((long long)c * 2 + (first ? 0 : 1)) * 2 + tile) * kPartFloats;
+      // A block's first segment is its part 0; only the item's first block can
+      // have begun before it.
+      const int first_part = attn_begin(share, c_first) < k.origin;
+      auto part = [&](int c) {
+        return parts + ((c * 2 + (c == c_first ? first_part : 0)) * 2 + tile) * (long long)kPartFloats;
       };
       float* mine = part(blockIdx.x);
 #pragma unroll

@@ -124,6 +124,13 @@ __device__ __forceinline__ int page_of(const b2g_kv_batch& b, const b2g_kv_cache
   return page;
 }
 
+// a * b / c; short work's products fit 32 bits, whose division is a fraction
+// of the 64-bit one's time.
+__device__ __forceinline__ long long mul_div(long long a, int b, long long c) {
+  const unsigned long long n = (unsigned long long)a * b;
+  if ((n | (unsigned long long)c) >> 32 == 0) return (unsigned)n / (unsigned)c;
+  return (long long)(n / (unsigned long long)c);
+}
 // ---------------------------------------------------------------------------
 // The attention kernels' work list.  An item is (sequence, tile of rows, k/v
 // head): the rows of a k/v head are its new tokens times its group of q
@@ -182,7 +189,7 @@ struct AttnWork {
       if (at < n) break;
       at -= n;
     }
-    it.h = (int)(at / (it.u_hi - it.u_lo));
+    it.h = (int)mul_div(at, 1, it.u_hi - it.u_lo);
     at -= (long long)it.h * (it.u_hi - it.u_lo);
     return it;
   }
@@ -214,6 +221,9 @@ struct AttnShare {
   long long at;                 // and the unit's offset in it
 };
 
+// The unit that block c's range begins with.
+__device__ __forceinline__ long long attn_begin(const AttnShare& s, int c) { return mul_div(s.total, c, s.blocks); }
+
 // Sums the list (all threads; sh: blockDim.x + 1 words) and finds the block's
 // range.  At least `least` units a block, so that short work is not cut finer
 // than the joining of its pieces is worth.
@@ -242,8 +252,8 @@ __device__ __forceinline__ AttnShare attn_share(const Work& w, int least, long l
   AttnShare r;
   r.total = total;
   r.blocks = (int)max(1LL, min((long long)gridDim.x, (total + least - 1) / least));
-  r.begin = (long long)blockIdx.x * total / r.blocks;
-  r.end = (long long)(blockIdx.x + 1) * total / r.blocks;
+  r.begin = attn_begin(r, blockIdx.x);
+  r.end = attn_begin(r, blockIdx.x + 1);
   if ((int)blockIdx.x >= r.blocks) r.begin = r.end = total;
   // The thread whose sequences hold `begin` tells the others.
   const long long from = before + incl - sum;
@@ -262,7 +272,9 @@ __device__ __forceinline__ AttnShare attn_share(const Work& w, int least, long l
 }
 // The block that has unit u.
 __device__ __forceinline__ int attn_owner(const AttnShare& s, long long u) {
-  return (int)(((u + 1) * s.blocks - 1) / s.total);
+  const unsigned long long n = (unsigned long long)(u + 1) * s.blocks - 1;
+  if ((n | (unsigned long long)s.total) >> 32 == 0) return (int)((unsigned)n / (unsigned)s.total);
+  return (int)(n / (unsigned long long)s.total);
 }
 
 }  // namespace b2g
