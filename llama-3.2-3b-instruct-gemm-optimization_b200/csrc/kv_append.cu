@@ -1,5 +1,7 @@
 // kv_append.cu -- new tokens' keys and values into a paged cache, with the
 // position rotation of k and q on the way.
+#include <algorithm>
+
 #include "serve.cuh"
 
 namespace b2g {
@@ -21,7 +23,7 @@ __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
   return r;
 }
 
-// One thread's piece of a head: 16 elements in two 16-byte chunks.
+// 16 bytes of a head.
 template <typename T>
 __device__ __forceinline__ void unpack8(uint4 v, float* f) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -38,109 +40,166 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
                     Act<T>::pack(f[6], f[7]));
 }
 
-// One block per row: its 16-element pieces (q heads, then k heads, then v
-// heads) over the threads.  Piece i of a rotated head uses the frequencies
-// 8i .. 8i + 7: the halves style pairs elements 8i.. with n_freq + 8i.., the
-// interleaved style the elements 16i .. 16i + 15 among themselves.
+// A block takes `rows` rows, a thread the same two 8-element chunks of a q, k
+// or v head in each of them, so what they are gets worked out once (by row and
+// chunk in turn the divisions took as long as the memory traffic).  The rows'
+// chunks are asked for before the rows' places and angles are worked out,
+// which take a chain of dependent reads.
+constexpr int kMostThreads = 384, kMaxRows = 4;
+
 template <typename T, bool FP8>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p) {
-  __shared__ float2 rot[128];
-  const int t = blockIdx.x;
-  const int lane = threadIdx.x & 31;
-  const int s = find_sequence(p.b, t, lane);
-  const SeqSpan q = seq_span(p.b, s);
-  if (t < q.first || t >= q.first + q.n) return;  // a row behind the last sequence
-  const int pos = q.ctx + (t - q.first);
+__global__ void __launch_bounds__(kMostThreads, 2) kv_append_kernel(const KvAppendParams p, int rows) {
+  __shared__ __align__(16) float2 rot[kMaxRows][64];
+  __shared__ long long slot_sh[kMaxRows];
+  __shared__ bool in_sh[kMaxRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row0 = blockIdx.x * rows, n_rows = min(rows, p.b.rows - row0);
   const int n_freq = p.a.n_freq;
-  if ((int)threadIdx.x < n_freq) rot[threadIdx.x] = sin_cos(pos, p.a.inv_freq[threadIdx.x]);
-  long long slot = -1;
-  if (pos >= 0) {
-    const int page_index = pos / p.c.page_size;
-    const int page = page_of(p.b, p.c, s, page_index, p.error);
-    if (page >= 0)
-      slot = page * p.c.stride_page + (long long)(pos - page_index * p.c.page_size) * p.c.stride_token;
-  }
-  __syncthreads();
   const int per_head = p.c.head_dim / 16;
-  const int n_q = p.a.q_heads * per_head, n_k = p.c.kv_heads * per_head;
-  for (int i = threadIdx.x; i < n_q + 2 * n_k; i += blockDim.x) {
-    const int kind = i < n_q ? 0 : i < n_q + n_k ? 1 : 2;
-    const int local = kind == 0 ? i : kind == 1 ? i - n_q : i - n_q - n_k;
-    const int head = local / per_head, piece = local - head * per_head;
-    if (kind != 0 && slot < 0) continue;
-    const bool turned = kind != 2 && piece * 8 < n_freq;
-    // Elements of the two chunks: the pair partner is n_freq away, or the
-    // next chunk; pieces behind the rotated part are plain neighbours.
-    const bool halves = turned && !p.a.interleaved;
-    const int e0 = halves ? 8 * piece : 16 * piece, e1 = halves ? e0 + n_freq : e0 + 8;
-    const T* src = kind == 0   ? static_cast<const T*>(p.a.q) + t * p.a.stride_q + head * p.a.stride_q_head
-                   : kind == 1 ? static_cast<const T*>(p.a.k) + t * p.a.stride_k + head * p.a.stride_k_head
-                               : static_cast<const T*>(p.a.v) + t * p.a.stride_v + head * p.a.stride_v_head;
-    float a[8], b[8];
-    unpack8<T>(*reinterpret_cast<const uint4*>(src + e0), a);
-    unpack8<T>(*reinterpret_cast<const uint4*>(src + e1), b);
-    if (turned) {
-      const float2* r = rot + 8 * piece;
-      if (halves) {
+  const int n_q = p.a.q_heads * per_head, n_k = p.c.kv_heads * per_head, per_row = n_q + 2 * n_k;
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int item = threadIdx.x; item < per_row || item == (int)threadIdx.x; item += blockDim.x) {
+    const bool mine = item < per_row;
+    const int kind = item < n_q ? 0 : item < n_q + n_k ? 1 : 2;
+    const int local = item - (kind == 0 ? 0 : kind == 1 ? n_q : n_q + n_k);
+    const int head = local / per_head, at = local - head * per_head;
+    // Two 8-element chunks half a head apart, so that a warp's accesses are
+    // whole lines (16 elements a thread in one run leave every 32-byte sector to
+    // two instructions: 90 us for 14,000 rows of 48 heads, 66 so).  Halves that are shorter
+    // than that pair over n_freq, and what is behind them is in runs of 16.
+    const bool halves_style = kind != 2 && !p.a.interleaved && n_freq > 0;
+    const bool halves = halves_style && at * 8 < n_freq;
+    const int e0 = halves_style && !halves ? 16 * at : 8 * at;
+    const int e1 = halves ? e0 + n_freq : halves_style ? e0 + 8 : e0 + p.c.head_dim / 2;
+    const bool pairs = kind != 2 && p.a.interleaved;
+    const bool pairs0 = pairs && e0 < 2 * n_freq, pairs1 = pairs && e1 < 2 * n_freq;
+    const T* src = static_cast<const T*>(kind == 0 ? p.a.q : kind == 1 ? p.a.k : p.a.v);
+    const long long step = kind == 0 ? p.a.stride_q : kind == 1 ? p.a.stride_k : p.a.stride_v;
+    src += row0 * step + head * (kind == 0 ? p.a.stride_q_head : kind == 1 ? p.a.stride_k_head : p.a.stride_v_head);
+    uint4 lo[kMaxRows], hi[kMaxRows];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = a[j], y = b[j];
-          a[j] = x * r[j].y - y * r[j].x;
-          b[j] = y * r[j].y + x * r[j].x;
+    for (int u = 0; u < kMaxRows; ++u)
+      if (mine && u < n_rows) {
+        lo[u] = *reinterpret_cast<const uint4*>(src + u * step + e0);
+        hi[u] = *reinterpret_cast<const uint4*>(src + u * step + e1);
+      }
+    if (item == (int)threadIdx.x) {  // the first time round: every thread is here
+      if (warp < n_rows) {
+        const int t = row0 + warp;
+        const int s = find_sequence(p.b, t, lane);
+        const SeqSpan q = seq_span(p.b, s);
+        const bool in = t >= q.first && t < q.first + q.n;  // else a row behind the last sequence
+        const int pos = q.ctx + (t - q.first);
+        for (int i = lane; in && i < n_freq; i += 32) rot[warp][i] = sin_cos(pos, p.a.inv_freq[i]);
+        long long slot = -1;
+        if (in && pos >= 0) {
+          const int page_index = pos / p.c.page_size;
+          const int page = page_of(p.b, p.c, s, page_index, p.error);
+          if (page >= 0)
+            slot = page * p.c.stride_page + (long long)(pos - page_index * p.c.page_size) * p.c.stride_token;
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x = a[2 * j], y = a[2 * j + 1];
-          a[2 * j] = x * r[j].y - y * r[j].x;
-          a[2 * j + 1] = y * r[j].y + x * r[j].x;
-          x = b[2 * j], y = b[2 * j + 1];
-          b[2 * j] = x * r[4 + j].y - y * r[4 + j].x;
-          b[2 * j + 1] = y * r[4 + j].y + x * r[4 + j].x;
+        if (lane == 0) {
+          slot_sh[warp] = slot;
+          in_sh[warp] = in;
         }
       }
+      __syncthreads();
     }
-    if (kind == 0) {
-      T* dst = static_cast<T*>(p.a.q_out) + t * p.a.stride_qo + head * p.a.stride_qo_head;
-      *reinterpret_cast<uint4*>(dst + e0) = pack8<T>(a);
-      *reinterpret_cast<uint4*>(dst + e1) = pack8<T>(b);
-      continue;
-    }
-    const long long at = slot + head * p.c.stride_head;
-    void* base = kind == 1 ? p.c.k : p.c.v;
+    float by = 1.0f;
     if constexpr (FP8) {
       const float* scale = kind == 1 ? p.c.k_scale : p.c.v_scale;
-      const float sc = scale ? scale[head] : 1.0f;
-      uint8_t* dst = static_cast<uint8_t*>(base) + at;
-      uint32_t w[4];
+      if (mine && kind != 0 && scale) by = 1.0f / scale[head];
+    }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        w[j] = e4m3_pair(a[4 * j] / sc, a[4 * j + 1] / sc) | e4m3_pair(a[4 * j + 2] / sc, a[4 * j + 3] / sc) << 16;
-        w[2 + j] = e4m3_pair(b[4 * j] / sc, b[4 * j + 1] / sc) | e4m3_pair(b[4 * j + 2] / sc, b[4 * j + 3] / sc) << 16;
+    for (int u = 0; u < kMaxRows; ++u) {
+      if (!mine || u >= n_rows) continue;
+      const long long slot = slot_sh[u];
+      if (!in_sh[u] || (kind != 0 && slot < 0)) continue;
+      float a[8], b[8];
+      unpack8<T>(lo[u], a);
+      unpack8<T>(hi[u], b);
+      if (halves) {
+        const float4* r4 = reinterpret_cast<const float4*>(rot[u] + e0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 r = r4[j];  // sine and cosine of two frequencies
+          float x = a[2 * j], y = b[2 * j];
+          a[2 * j] = x * r.y - y * r.x;
+          b[2 * j] = y * r.y + x * r.x;
+          x = a[2 * j + 1], y = b[2 * j + 1];
+          a[2 * j + 1] = x * r.w - y * r.z;
+          b[2 * j + 1] = y * r.w + x * r.z;
+        }
       }
-      *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(dst + e1) = make_uint2(w[2], w[3]);
-    } else {
-      T* dst = static_cast<T*>(base) + at;
-      *reinterpret_cast<uint4*>(dst + e0) = pack8<T>(a);
-      *reinterpret_cast<uint4*>(dst + e1) = pack8<T>(b);
+      auto turn_pairs = [&](float (&v)[8], int e) {
+        const float4* r4 = reinterpret_cast<const float4*>(rot[u] + e / 2);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float4 r = r4[j];
+          float x = v[4 * j], y = v[4 * j + 1];
+          v[4 * j] = x * r.y - y * r.x;
+          v[4 * j + 1] = y * r.y + x * r.x;
+          x = v[4 * j + 2], y = v[4 * j + 3];
+          v[4 * j + 2] = x * r.w - y * r.z;
+          v[4 * j + 3] = y * r.w + x * r.z;
+        }
+      };
+      if (pairs0) turn_pairs(a, e0);
+      if (pairs1) turn_pairs(b, e1);
+      if (kind == 0) {
+        T* dst = static_cast<T*>(p.a.q_out) + (row0 + u) * p.a.stride_qo + head * p.a.stride_qo_head;
+        *reinterpret_cast<uint4*>(dst + e0) = pack8<T>(a);
+        *reinterpret_cast<uint4*>(dst + e1) = pack8<T>(b);
+        continue;
+      }
+      const long long to = slot + head * p.c.stride_head;
+      void* cache = kind == 1 ? p.c.k : p.c.v;
+      if constexpr (FP8) {
+        uint8_t* dst = static_cast<uint8_t*>(cache) + to;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          w[j] = e4m3_pair(a[4 * j] * by, a[4 * j + 1] * by) | e4m3_pair(a[4 * j + 2] * by, a[4 * j + 3] * by) << 16;
+          w[2 + j] = e4m3_pair(b[4 * j] * by, b[4 * j + 1] * by) | e4m3_pair(b[4 * j + 2] * by, b[4 * j + 3] * by) << 16;
+        }
+        *reinterpret_cast<uint2*>(dst + e0) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(dst + e1) = make_uint2(w[2], w[3]);
+      } else {
+        T* dst = static_cast<T*>(cache) + to;
+        *reinterpret_cast<uint4*>(dst + e0) = pack8<T>(a);
+        *reinterpret_cast<uint4*>(dst + e1) = pack8<T>(b);
+      }
     }
   }
 }
 
+template <typename T, bool FP8>
+cudaError_t launch(const KvAppendParams& p, int num_sms, cudaStream_t stream) {
+  // Rows a block: one while the rows are few (latency), else as many as keep
+  // four blocks an SM.
+  const int rows = std::min(kMaxRows, std::max(1, p.b.rows / (4 * num_sms)));
+  const int per_row = (p.a.q_heads + 2 * p.c.kv_heads) * p.c.head_dim / 16;
+  const int threads = std::min(kMostThreads, std::max(32 * kMaxRows, (per_row + 31) / 32 * 32));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.b.rows + rows - 1) / rows);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_append_kernel<T, FP8>, p, rows);
+}
+
 }  // namespace
 
-cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t stream) {
+cudaError_t launch_kv_append(const KvAppendParams& p, int num_sms, cudaStream_t stream) {
   const bool fp8 = p.c.dtype == B2G_DTYPE_FP8_E4M3;
-  const dim3 grid(p.b.rows), block(256);
-  if (p.a.dtype == B2G_DTYPE_BF16) {
-    if (fp8) kv_append_kernel<__nv_bfloat16, true><<<grid, block, 0, stream>>>(p);
-    else kv_append_kernel<__nv_bfloat16, false><<<grid, block, 0, stream>>>(p);
-  } else {
-    if (fp8) kv_append_kernel<__half, true><<<grid, block, 0, stream>>>(p);
-    else kv_append_kernel<__half, false><<<grid, block, 0, stream>>>(p);
-  }
-  return cudaGetLastError();
+  if (p.a.dtype == B2G_DTYPE_BF16)
+    return fp8 ? launch<__nv_bfloat16, true>(p, num_sms, stream) : launch<__nv_bfloat16, false>(p, num_sms, stream);
+  return fp8 ? launch<__half, true>(p, num_sms, stream) : launch<__half, false>(p, num_sms, stream);
 }
 
 }  // namespace b2g

@@ -92,7 +92,7 @@ struct KvAppendParams {
   b2g_kv_batch b;
   int* error;
 };
-cudaError_t launch_kv_append(const KvAppendParams& p, cudaStream_t stream);
+cudaError_t launch_kv_append(const KvAppendParams& p, int num_sms, cudaStream_t stream);
 
 struct AttnParams {
   b2g_attn_args a;

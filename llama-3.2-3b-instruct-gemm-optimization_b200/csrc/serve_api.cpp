@@ -245,10 +245,12 @@ b2g_status b2g_kv_append(const b2g_kv_append_args* a, const b2g_kv_cache* c, con
   int dev = -1;
   st = current_device(&dev);
   if (st != B2G_OK) return st;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return B2G_ERR_CUDA;
   KvAppendParams p = {*a, *c, *b, registered_error_word(dev)};
   if (!p.a.inv_freq) p.a.n_freq = 0;
   if (!p.error) return B2G_ERR_CUDA;
-  return cuda_status(launch_kv_append(p, cu(stream)));
+  return cuda_status(launch_kv_append(p, sms, cu(stream)));
 }
 
 b2g_status b2g_attn_create(const b2g_attn_fields* f, b2g_attn** out) {
