@@ -540,11 +540,12 @@ def _launch_stream(stream, device, tensors):
     import torch
     if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
         raise ValueError(f"tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    index = device.index
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"tensors on {device} and {t.device}")
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device.index)
+        return torch._C._cuda_getCurrentRawStream(index)
     if stream.device != device:
         raise ValueError(f"tensors on {device}, a stream of {stream.device}")
     return stream.cuda_stream

@@ -199,13 +199,21 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
 // One persistent CTA per SM.  Warp 0 streams 128-byte k blocks of both
 // operands through a ring of stages (TMA, 128-byte swizzle, zeros outside the
 // matrices), warp 1 issues tcgen05.mma.kind::i8 into one of two accumulators
-// in tensor memory, warps 2..5 drain the other one.  Work is cut as whole
-// tiles where they fill the SMs, else as equal ranges of k blocks ("units"):
-// a range's tiles at its two ends are shared with other CTAs, which all add
-// their int32 sums into the workspace (integers: the order does not matter);
-// the last to arrive finishes the tile and leaves zeros behind.
+// in tensor memory, warps 2..5 drain the other one.
+// Many tokens take a deep tile instead: 2 x 128 channels by up to 256 tokens,
+// which moves two thirds of the bytes a product from L2 (what bounds the narrow
+// one: 240 clocks an MMA of 128 x 256 where the tensor cores need 128), but
+// fills tensor memory with one accumulator, drained by eight warps between
+// tiles.
+// Work is cut in one of three ways.  Whole tiles, where they fill the SMs.  A
+// cluster of 2, 4 or 8 CTAs a tile, where that many fit: each takes a part of K
+// and leaves its int32 sums in its shared memory, and each finishes a part of
+// the columns from everybody's (one token by 8192 x 4096: 13 us, 18.6 through
+// global memory).  Else equal ranges of k blocks ("units"): a range's tiles at
+// its two ends are shared with other CTAs, which all add their int32 sums into
+// the workspace (integers: the order does not matter); the last to arrive
+// finishes the tile and leaves zeros behind.
 // ---------------------------------------------------------------------------
-constexpr int kI8Threads = 192;
 constexpr int kI8MaxStages = 12;
 constexpr int kKBlock = 128;
 constexpr int kChTile = 128;
@@ -216,6 +224,7 @@ struct I8Tc {
   I8Params p;
   int bn, stages, kb, tok_tiles, tiles, whole;
   int cluster;          // CTAs a tile (1: none)
+  int acc_cols;         // tensor-memory columns of an accumulator
   int tmem_cols, after_quantiser;
   long long units;
   long long slot_ints;  // int32 words of one partial
@@ -266,15 +275,19 @@ __device__ __forceinline__ int i8_owner(const I8Tc& t, long long u) {
 }
 
 // The scaled sum, or SiLU(gate) * up.
-template <int PLANES>
-__device__ __forceinline__ float i8_value(int acc, int acc_up, const float (&sw)[PLANES], float sx) {
-  const float v = (float)acc * sw[0] * sx;
-  if constexpr (PLANES == 1) return v;
-  return v / (1.0f + __expf(-v)) * ((float)acc_up * sw[PLANES - 1] * sx);
+template <bool GATE>
+__device__ __forceinline__ float i8_value(int acc, int acc_up, float sw, float sw_up, float sx) {
+  const float v = (float)acc * sw * sx;
+  if constexpr (!GATE) return v;
+  return v / (1.0f + __expf(-v)) * ((float)acc_up * sw_up * sx);
 }
 
-template <typename T, int PLANES>
-__global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_constant__ I8Tc t) {
+// PLANES 128-row weight tiles a stage: gate and up (GATE), or two channel tiles.
+template <typename T, int PLANES, bool GATE, bool DEEP>
+__global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const __grid_constant__ I8Tc t) {
+  constexpr int kEpi = DEEP ? 256 : 128;  // epilogue threads
+  constexpr int kBufs = DEEP ? 1 : 2;     // accumulators
+  constexpr int kChannels = GATE ? kChTile : PLANES * kChTile;  // of a tile
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kI8MaxStages], empty[kI8MaxStages], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_base_sh;
@@ -290,7 +303,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 128);
+      mbar_init(&acc_empty[i], kEpi);
     }
     mbar_init(&drain, 1);
     fence_mbarrier_init();
@@ -300,7 +313,6 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
-  pdl_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -310,8 +322,8 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         uint8_t* dst = ring + stage * stage_bytes;
 #pragma unroll
         for (int pl = 0; pl < PLANES; ++pl)
-          tma_load_2d(dst + pl * kChTile * kKBlock, &t.mw, k * kKBlock, pl * t.p.n + s.tile / t.tok_tiles * kChTile,
-                      &full[stage]);
+          tma_load_2d(dst + pl * kChTile * kKBlock, &t.mw, k * kKBlock,
+                      pl * (GATE ? t.p.n : kChTile) + s.tile / t.tok_tiles * kChannels, &full[stage]);
       };
       auto load_x = [&](int stage, const I8Seg& s, int k) {
         tma_load_2d(ring + stage * stage_bytes + PLANES * kChTile * kKBlock, &t.mx, k * kKBlock,
@@ -359,8 +371,8 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
       int i = 0, n = 0;
       bool ok = true;
       while (ok && s.next(t)) {
-        const int buf = n & 1;
-        if (!mbar_wait_spin(&acc_empty[buf], ((n >> 1) & 1) ^ 1)) {
+        const int buf = n % kBufs;
+        if (!mbar_wait_spin(&acc_empty[buf], ((n / kBufs) & 1) ^ 1)) {
           *t.error = kErrEmptyWait;
           ok = false;
           break;
@@ -379,7 +391,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl) {
             const uint64_t da = smem_desc_sw128(a0 + pl * kChTile * kKBlock, 16, 1024);
-            const uint32_t d = tmem + (buf * PLANES + pl) * t.bn;
+            const uint32_t d = tmem + (buf * PLANES + pl) * t.acc_cols;
 #pragma unroll
             for (int j = 0; j < 4; ++j)  // 32 k an instruction: 2 units of 16 bytes
               mma_i8_ss(d, da + 2 * j, db + 2 * j, idesc, k > s.k0 || j > 0);
@@ -396,6 +408,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
     }
   } else {
     pdl_wait();
+    pdl_launch_dependents();  // behind the wait: what came before this launch is complete
     const int quad = warp & 3, et = threadIdx.x - 64;
     const int ch = quad * 32 + lane;  // channel in the tile
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
@@ -404,27 +417,36 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
     s.begin(t);
     int n = 0;
     while (s.next(t)) {
-      const int buf = n & 1;
-      const int tok0 = s.tile % t.tok_tiles * t.bn, j = s.tile / t.tok_tiles * kChTile + ch;
+      const int buf = n % kBufs;
+      const int tok0 = s.tile % t.tok_tiles * t.bn, j = s.tile / t.tok_tiles * kChannels + ch;
       const int cols = min(t.bn, p.m - tok0);
       const bool split = t.cluster == 1 && (s.k0 != 0 || s.k1 != t.kb);
       float sw[PLANES];
 #pragma unroll
-      for (int pl = 0; pl < PLANES; ++pl) sw[pl] = j < p.n ? p.sw[pl * p.n + j] : 0.f;
+      for (int pl = 0; pl < PLANES; ++pl) {
+        const int c = j + (GATE ? 0 : pl * kChTile);
+        sw[pl] = c < p.n ? p.sw[(GATE ? pl * p.n : 0) + c] : 0.f;
+      }
       // Everything the epilogue reads from global memory is asked for before
       // the accumulator is waited for (residual rows: a chunk ahead).
       float* sx = sx_sh[n & 1];
-      for (int c = et; c < cols; c += 128) sx[c] = p.sx[tok0 + c];
-      const T* res_col = p.residual && j < p.n ? static_cast<const T*>(p.residual) + tok0 * p.ldr + j : nullptr;
-      T res[32];
+      for (int c = et; c < cols; c += kEpi) sx[c] = p.sx[tok0 + c];
+      // 32 columns at a time (two groups of warps take them in turn).
+      const int first = DEEP ? 32 * (et >> 7) : 0;
+      constexpr int kStepCols = 32 * (kEpi / 128), kOuts = GATE ? 1 : PLANES;
+      T res[kOuts][32];
       auto load_residual = [&](int c0) {
-        if (!res_col) return;
+        if (!p.residual) return;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) res[c] = res_col[min(c0 + c, cols - 1) * p.ldr];
+        for (int o = 0; o < kOuts; ++o) {
+          const T* col = static_cast<const T*>(p.residual) + tok0 * p.ldr + min(j + o * kChTile, p.n - 1);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) res[o][c] = col[min(c0 + c, cols - 1) * p.ldr];
+        }
       };
-      if (t.cluster == 1) load_residual(0);
-      named_sync(1, 128);
-      if (!mbar_wait_spin(&acc_full[buf], (n >> 1) & 1)) {
+      if (t.cluster == 1) load_residual(first);
+      named_sync(1, kEpi);
+      if (!mbar_wait_spin(&acc_full[buf], (n / kBufs) & 1)) {
         *t.error = kErrFullWait;
         break;
       }
@@ -433,14 +455,14 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
       // a clamped row) and not stored, so that no load waits on a branch.
       bool finish = true;
       int* sums = nullptr;
-      if (t.cluster > 1) {
+      if (!DEEP && t.cluster > 1) {
         // The ring is free: every MMA that read it is done.  [plane][column][channel].
         int* mine = reinterpret_cast<int*>(ring);
         for (int c0 = 0; c0 < cols; c0 += 32) {
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl) {
             uint32_t r[32];
-            tmem_ld32(lane_addr + (buf * PLANES + pl) * t.bn + c0, r);
+            tmem_ld32(lane_addr + (buf * PLANES + pl) * t.acc_cols + c0, r);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 32; ++c) mine[(pl * t.bn + c0 + c) * kChTile + ch] = (int)r[c];
@@ -448,7 +470,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         }
         break;  // the only segment; the rest is behind the cluster's barrier
       }
-      if (split) {
+      if (!DEEP && split) {
         const int c_first = i8_owner(t, (long long)s.tile * t.kb);
         const int c_last = i8_owner(t, (long long)(s.tile + 1) * t.kb - 1);
         sums = t.partials + c_first * t.slot_ints + ch;
@@ -456,7 +478,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl) {
             uint32_t r[32];
-            tmem_ld32(lane_addr + (buf * PLANES + pl) * t.bn + c0, r);
+            tmem_ld32(lane_addr + (buf * PLANES + pl) * t.acc_cols + c0, r);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 32; ++c)
@@ -475,10 +497,10 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         __threadfence();
       }
       if (finish) {
-        for (int c0 = 0; c0 < cols; c0 += 32) {
+        for (int c0 = first; c0 < cols; c0 += kStepCols) {
           uint32_t r[PLANES][32];
           const int rows = cols - c0;  // of this chunk, if less than 32
-          if (split) {
+          if (!DEEP && split) {
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
@@ -489,24 +511,28 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
               for (int c = 0; c < 32; ++c) __stcg(sums + (pl * t.bn + c0 + c) * kChTile, 0);
           } else {
 #pragma unroll
-            for (int pl = 0; pl < PLANES; ++pl) tmem_ld32(lane_addr + (buf * PLANES + pl) * t.bn + c0, r[pl]);
+            for (int pl = 0; pl < PLANES; ++pl) tmem_ld32(lane_addr + (buf * PLANES + pl) * t.acc_cols + c0, r[pl]);
             tmem_wait_ld();
           }
-          T* to = static_cast<T*>(p.y) + (tok0 + c0) * p.ldy + j;
-          T out[32];
+          T out[kOuts][32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            float v = i8_value<PLANES>((int)r[0][c], (int)r[PLANES - 1][c], sw, sx[c0 + c]);
-            if (res_col) v += Act<T>::to_float(res[c]);
-            out[c] = Act<T>::from_float(v);
-          }
+          for (int o = 0; o < kOuts; ++o)
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              float v = i8_value<GATE>((int)r[o][c], (int)r[PLANES - 1][c], sw[o], sw[PLANES - 1], sx[c0 + c]);
+              if (p.residual) v += Act<T>::to_float(res[o][c]);
+              out[o][c] = Act<T>::from_float(v);
+            }
           // Loaded before the stores: residual and y may be one buffer, but a
           // chunk's rows are its own.
-          load_residual(c0 + 32);
-          if (j < p.n) {
+          load_residual(c0 + kStepCols);
+#pragma unroll
+          for (int o = 0; o < kOuts; ++o) {
+            if (j + o * kChTile >= p.n) continue;
+            T* to = static_cast<T*>(p.y) + (tok0 + c0) * p.ldy + j + o * kChTile;
 #pragma unroll
             for (int c = 0; c < 32; ++c)
-              if (c < rows) to[c * p.ldy] = out[c];
+              if (c < rows) to[c * p.ldy] = out[o][c];
           }
         }
       }
@@ -516,7 +542,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
     }
   }
   __syncwarp();
-  if (t.cluster > 1) {
+  if (!DEEP && t.cluster > 1) {
     // This CTA's columns of the tile, from all the cluster's sums.  What comes
     // from global memory is asked for before the barrier.
     const I8Params& p = t.p;
@@ -554,7 +580,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) i8_product_kernel(const __grid_
         T out[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          float v = i8_value<PLANES>(acc[0][c], acc[PLANES - 1][c], sw, sx_sh[0][c0 + min(c, n - 1)]);
+          float v = i8_value<GATE>(acc[0][c], acc[PLANES - 1][c], sw[0], sw[PLANES - 1], sx_sh[0][c0 + min(c, n - 1)]);
           if (p.residual) v += Act<T>::to_float(res[c]);
           out[c] = Act<T>::from_float(v);
         }
@@ -598,13 +624,25 @@ int i8_bn(int m, int planes) {
   return up32((m + tiles - 1) / tiles);
 }
 
-template <typename T, int PLANES>
+template <typename T, int PLANES, bool GATE, bool DEEP>
 cudaError_t launch_product(const I8Tc& t, int grid, int smem, cudaStream_t stream) {
   static std::atomic<uint64_t> allowed{0};  // devices whose limit is set
-  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(i8_product_kernel<T, PLANES>), kI8SmemBytes, &allowed);
+  const auto kernel = i8_product_kernel<T, PLANES, GATE, DEEP>;
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), kI8SmemBytes, &allowed);
   if (e != cudaSuccess) return e;
-  return launch_after(i8_product_kernel<T, PLANES>, dim3(grid), dim3(kI8Threads), smem, t.cluster, stream, t);
+  return launch_after(kernel, dim3(grid), dim3(DEEP ? 320 : 192), smem, t.cluster, stream, t);
 }
+
+template <typename T>
+cudaError_t launch_typed(const I8Tc& t, bool deep, int grid, int smem, cudaStream_t stream) {
+  if (t.p.planes == 2)
+    return deep ? launch_product<T, 2, true, true>(t, grid, smem, stream)
+                : launch_product<T, 2, true, false>(t, grid, smem, stream);
+  return deep ? launch_product<T, 2, false, true>(t, grid, smem, stream)
+              : launch_product<T, 1, false, false>(t, grid, smem, stream);
+}
+
+int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 }  // namespace
 
@@ -640,22 +678,45 @@ cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int
   I8Tc t;
   t.p = p;
   t.bn = i8_bn(p.m, p.planes);
-  const int stage_bytes = (p.planes * kChTile + t.bn) * kKBlock;
+  t.tok_tiles = div_up(p.m, t.bn);
+  t.tiles = t.tok_tiles * div_up(p.n, kChTile);
+  // Whole tiles take (waves of tiles) x (columns of a tile's products).  A deep
+  // tile has twice a narrow one's rows (or, gate||up, the narrow one's planes
+  // and up to twice its columns), at 0.7 of the time for each product; its
+  // columns (a multiple of 16) are chosen for the fewest waves x columns.
+  const int deep_ch = div_up(p.n, p.planes == 2 ? kChTile : 2 * kChTile);
+  long long deep_cost = 0;
+  int deep_bn = 0;
+  for (int bn = 144; bn <= 256; bn += 16) {
+    const long long cost = (long long)div_up((long long)deep_ch * div_up(p.m, bn), num_sms) * bn;
+    if (!deep_bn || cost <= deep_cost) deep_cost = cost, deep_bn = bn;
+  }
+  const long long narrow_cost = (long long)div_up(t.tiles, num_sms) * t.bn;
+  const bool deep = deep_cost * (p.planes == 2 ? 10 : 20) * 7 < narrow_cost * 100 && t.tiles >= num_sms;
+  if (deep) {
+    t.bn = deep_bn;
+    t.tok_tiles = div_up(p.m, t.bn);
+    t.tiles = t.tok_tiles * deep_ch;
+  }
+  const int stage_tiles = deep ? 2 : p.planes;
+  const int stage_bytes = (stage_tiles * kChTile + t.bn) * kKBlock;
   t.stages = std::min(kI8MaxStages, (kI8SmemBytes - 1024) / stage_bytes);
-  if (t.bn * p.planes <= 64 && t.stages * stage_bytes > 100 * 1024) t.stages = 100 * 1024 / stage_bytes;
-  t.kb = (p.k + kKBlock - 1) / kKBlock;
-  t.tok_tiles = (p.m + t.bn - 1) / t.bn;
-  t.tiles = t.tok_tiles * ((p.n + kChTile - 1) / kChTile);
+  // Narrow tiles leave room for a second CTA, the next launch's: it sets
+  // itself up while this one runs (12.9 us a product of 1 x 8192 x 4096
+  // instead of 14.1), and 100 KB in flight still hide the latency.
+  if (t.bn * stage_tiles <= 64) t.stages = std::min(t.stages, 100 * 1024 / stage_bytes);
+  t.kb = div_up(p.k, kKBlock);
   t.units = (long long)t.tiles * t.kb;
+  t.acc_cols = deep ? 256 : t.bn;
   t.tmem_cols = 32;
-  while (t.tmem_cols < 2 * p.planes * t.bn) t.tmem_cols *= 2;
+  while (t.tmem_cols < (deep ? 1 : 2) * stage_tiles * t.acc_cols) t.tmem_cols *= 2;
   t.slot_ints = (long long)p.planes * t.bn * kChTile;
   t.counters = counters;
   t.partials = partials;
   t.error = error;
   // Whole tiles where the last wave leaves at most a tenth of the SMs' time idle.
-  const int waves = (t.tiles + num_sms - 1) / num_sms;
-  t.whole = t.tiles * 10LL >= (long long)waves * num_sms * 9;
+  const int waves = div_up(t.tiles, num_sms);
+  t.whole = deep || t.tiles * 10LL >= (long long)waves * num_sms * 9;
   int grid = (int)std::min<long long>(t.whole ? t.tiles : t.units, num_sms);
   // A cluster a tile where at least two CTAs fit for every tile (a GPC holds
   // 16 SMs or more, so sizes up to 8 pack without much loss).
@@ -668,11 +729,8 @@ cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int
       !encode_rows(&t.mx, p.x, p.m, p.k, p.ldx, t.bn))
     return cudaErrorInvalidValue;
   const int smem = t.stages * stage_bytes + 1024;
-  if (p.bf16)
-    return p.planes == 2 ? launch_product<__nv_bfloat16, 2>(t, grid, smem, stream)
-                         : launch_product<__nv_bfloat16, 1>(t, grid, smem, stream);
-  return p.planes == 2 ? launch_product<__half, 2>(t, grid, smem, stream)
-                       : launch_product<__half, 1>(t, grid, smem, stream);
+  return p.bf16 ? launch_typed<__nv_bfloat16>(t, deep, grid, smem, stream)
+                : launch_typed<__half>(t, deep, grid, smem, stream);
 }
 
 }  // namespace b2g

@@ -56,10 +56,12 @@ def check_product(b2g, m, n, k, dtype="fp16", fuse=0, seed=3, ldx=None, op=None,
 
 # (tokens, channels, k): one k block, k that is no multiple of the block or of
 # 16, channels that end inside a tile, each way of cutting the work (whole
-# tiles, clusters of 2, 4, 8, shared ranges), token tiles of 32 to 256.
+# tiles, clusters of 2, 4, 8, shared ranges, deep tiles), token tiles of 32 to
+# 256.
 SHAPES = [(1, 1, 1), (1, 128, 128), (2, 17, 40), (5, 100, 1000), (32, 128, 256), (33, 129, 129), (1, 4096, 2048),
           (8, 1024, 8192), (64, 2048, 512), (100, 8192, 256), (127, 300, 4096), (256, 19000, 128), (257, 513, 77),
-          (300, 9600, 1024), (517, 1000, 640), (1, 20000, 64), (700, 5000, 300)]
+          (300, 9600, 1024), (517, 1000, 640), (1, 20000, 64), (700, 5000, 300),
+          (1000, 6000, 700), (1500, 5000, 333), (2049, 4100, 130)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
