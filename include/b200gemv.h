@@ -548,7 +548,7 @@ typedef struct b2g_attn b2g_attn;
 typedef struct {
   const void* q;
   int64_t stride_q, stride_q_head;
-  void* out;
+  void* out; /* may be q itself (same strides): a row's q is read before its out is written */
   int64_t stride_o, stride_o_head;
   float* lse; /* [rows, q_heads] natural log of the sum of exp(scale * q . k), or NULL */
   float scale;

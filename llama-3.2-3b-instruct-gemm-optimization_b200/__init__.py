@@ -538,9 +538,11 @@ def _act_code(t):
 def _launch_stream(stream, device, tensors):
     """The raw stream to launch on, once every tensor is on the current device."""
     import torch
-    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    if device.type != "cuda":
+        raise ValueError(f"tensors on {device}: expected a CUDA device")
     index = device.index
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise ValueError(f"tensors on {device} and {t.device}")
@@ -826,7 +828,8 @@ class AttnOp:
 
     def enqueue(self, q, cache, q_start, seq_lens, page_table, max_q=None, scale=None, window: int = 0, out=None,
                 lse=None, workspace=None, stream=None):
-        """out [rows, q_heads, dim] of q; lse [rows, q_heads] float32 receives the log-sums.
+        """out [rows, q_heads, dim] of q (may be q itself); lse [rows, q_heads]
+        float32 receives the log-sums.
 
         max_q: the most new tokens of one sequence (None: unknown), a hint that
         picks the kernel.  scale: default 1 / sqrt(dim).  window: a token sees
@@ -853,3 +856,47 @@ class AttnOp:
         if status:
             check(status, "b2g_attn_enqueue")
         return out
+
+
+class AttentionBlock:
+    """The attention half of a decoder layer, beside Stack's MLP half: h (updated
+    in place) += out(attention(append(qkv(RMSNorm(h))))), for any number of new
+    tokens of each sequence -- a decode step, a prompt chunk, or both.  Rows of
+    h behind the last sequence are computed on, from nothing of use.
+
+    wqkv: codes [(q_heads + 2 * kv_heads) * head_dim, hidden] and scales, q
+    heads first, then k, then v; wo: codes [hidden, q_heads * head_dim] and
+    scales; as quantize_i8_weights leaves them.  gamma: the norm's weights or
+    None (1).  inv_freq: the rotation's frequencies (float32, [head_dim / 2]).
+    """
+
+    def __init__(self, hidden: int, q_heads: int, kv_heads: int, head_dim: int, max_rows: int, max_batch: int, wqkv, wo,
+                 inv_freq, gamma=None, rms_eps: float = 1e-5, dtype="fp16", cache_dtype=None,
+                 interleaved: bool = False):
+        import torch
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        heads = q_heads + 2 * kv_heads
+        self.qkv = I8Op(hidden, heads * head_dim, max_rows, FUSE_RMSNORM_INPUT, dtype)
+        self.attn = AttnOp(q_heads, kv_heads, head_dim, max_batch, dtype, cache_dtype)
+        self.out = I8Op(q_heads * head_dim, hidden, max_rows, FUSE_RESIDUAL_ADD, dtype)
+        self.wqkv, self.wo, self.inv_freq, self.gamma = wqkv, wo, inv_freq, gamma
+        self.rms_eps, self.interleaved = rms_eps, interleaved
+        self._rows = torch.empty((max_rows, heads, head_dim), dtype=self.qkv._type, device=wqkv[0].device)
+
+    def workspace(self, device="cuda", stream=None):
+        """The three ops' workspaces.  Calls that can overlap need their own,
+        and a block of their own (it holds the rows between its ops)."""
+        return tuple(op.workspace(device, stream) for op in (self.qkv, self.attn, self.out))
+
+    def enqueue(self, h, cache, q_start, seq_lens, page_table, workspace, max_q=None, window: int = 0, stream=None):
+        m = h.shape[0]
+        rows = self._rows[:m]
+        self.qkv.enqueue(h, *self.wqkv, y=rows.view(m, -1), workspace=workspace[0], gamma=self.gamma,
+                         rms_eps=self.rms_eps, stream=stream)
+        q, k, v = rows.split((self.q_heads, self.kv_heads, self.kv_heads), dim=1)
+        kv_append(k, v, cache, q_start, seq_lens, page_table, q=q, inv_freq=self.inv_freq, interleaved=self.interleaved,
+                  stream=stream)
+        # Each head's result over its q: no row needs another row's q.
+        self.attn.enqueue(q, cache, q_start, seq_lens, page_table, max_q=max_q, window=window, out=q,
+                          workspace=workspace[1], stream=stream)
+        return self.out.enqueue(q.flatten(1), *self.wo, y=h, residual=h, workspace=workspace[2], stream=stream)

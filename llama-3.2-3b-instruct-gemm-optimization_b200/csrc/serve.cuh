@@ -86,7 +86,7 @@ struct SeqSpan {
   int first, n;  // its rows are first .. first + n - 1
   int ctx;       // position of its row 0 (negative: more rows than the length counts)
 };
-__device__ __forceinline__ SeqSpan seq_span(const b2g_kv_batch& b, int s) {
+__host__ __device__ __forceinline__ SeqSpan seq_span(const b2g_kv_batch& b, int s) {
   SeqSpan r;
   const int lo = min(max(b.q_start[s], 0), b.rows);
   const int hi = min(max(b.q_start[s + 1], lo), b.rows);
@@ -113,7 +113,7 @@ __device__ __forceinline__ int find_sequence(const b2g_kv_batch& b, int t, int l
 
 // The page of token position pos of sequence s, or -1 (with the error word
 // set) where the table or the cache does not have it.
-__device__ __forceinline__ int page_of(const b2g_kv_batch& b, const b2g_kv_cache& c, int s, int page_index,
+__host__ __device__ __forceinline__ int page_of(const b2g_kv_batch& b, const b2g_kv_cache& c, int s, int page_index,
                                        int* error) {
   int page = -1;
   if (page_index < b.max_pages) page = b.page_table[(long long)s * b.page_table_stride + page_index];
@@ -126,7 +126,7 @@ __device__ __forceinline__ int page_of(const b2g_kv_batch& b, const b2g_kv_cache
 
 // a * b / c; short work's products fit 32 bits, whose division is a fraction
 // of the 64-bit one's time.
-__device__ __forceinline__ long long mul_div(long long a, int b, long long c) {
+__host__ __device__ __forceinline__ long long mul_div(long long a, int b, long long c) {
   const unsigned long long n = (unsigned long long)a * b;
   if ((n | (unsigned long long)c) >> 32 == 0) return (unsigned)n / (unsigned)c;
   return (long long)(n / (unsigned long long)c);
@@ -152,11 +152,11 @@ template <int ROWS, int UNIT>
 struct AttnWork {
   const AttnParams& p;
   int cap;  // tokens that the page table has entries for
-  __device__ __forceinline__ explicit AttnWork(const AttnParams& p_) : p(p_) {
+  __host__ __device__ __forceinline__ explicit AttnWork(const AttnParams& p_) : p(p_) {
     cap = (int)min((long long)p_.b.max_pages * p_.c.page_size, 0x7fffffffLL - UNIT);
   }
-  __device__ __forceinline__ int tiles(const SeqSpan& s) const { return (s.n * p.group + ROWS - 1) / ROWS; }
-  __device__ __forceinline__ void range(AttnItem& it) const {
+  __host__ __device__ __forceinline__ int tiles(const SeqSpan& s) const { return (s.n * p.group + ROWS - 1) / ROWS; }
+  __host__ __device__ __forceinline__ void range(AttnItem& it) const {
     const int first = it.tile * ROWS / p.group;
     const int last = min(it.s.n - 1, (it.tile * ROWS + ROWS - 1) / p.group);
     if (it.s.ctx + last >= cap) *p.error = kErrBadPage;
@@ -166,7 +166,7 @@ struct AttnWork {
     it.u_hi = max((it.hi + UNIT - 1) / UNIT, it.u_lo + 1);
   }
   // Units of a sequence's items.
-  __device__ __forceinline__ long long units(int b) const {
+  __host__ __device__ __forceinline__ long long units(int b) const {
     AttnItem it;
     it.s = seq_span(p.b, b);
     long long n = 0;
@@ -179,7 +179,7 @@ struct AttnWork {
   }
   // The item that holds unit `at` of sequence b; `at` becomes the unit's
   // offset in the item.
-  __device__ __forceinline__ AttnItem find(int b, long long& at) const {
+  __host__ __device__ __forceinline__ AttnItem find(int b, long long& at) const {
     AttnItem it;
     it.b = b;
     it.s = seq_span(p.b, b);
@@ -194,7 +194,7 @@ struct AttnWork {
     return it;
   }
   // The next item in order (false: none left).
-  __device__ __forceinline__ bool next(AttnItem& it) const {
+  __host__ __device__ __forceinline__ bool next(AttnItem& it) const {
     if (++it.h < p.c.kv_heads) return true;
     it.h = 0;
     if (++it.tile < tiles(it.s)) {
@@ -222,7 +222,7 @@ struct AttnShare {
 };
 
 // The unit that block c's range begins with.
-__device__ __forceinline__ long long attn_begin(const AttnShare& s, int c) { return mul_div(s.total, c, s.blocks); }
+__host__ __device__ __forceinline__ long long attn_begin(const AttnShare& s, int c) { return mul_div(s.total, c, s.blocks); }
 
 // Sums the list (all threads; sh: blockDim.x + 1 words) and finds the block's
 // range.  At least `least` units a block, so that short work is not cut finer
@@ -271,7 +271,7 @@ __device__ __forceinline__ AttnShare attn_share(const Work& w, int least, long l
   return r;
 }
 // The block that has unit u.
-__device__ __forceinline__ int attn_owner(const AttnShare& s, long long u) {
+__host__ __device__ __forceinline__ int attn_owner(const AttnShare& s, long long u) {
   const unsigned long long n = (unsigned long long)(u + 1) * s.blocks - 1;
   if ((n | (unsigned long long)s.total) >> 32 == 0) return (int)((unsigned)n / (unsigned)s.total);
   return (int)(n / (unsigned long long)s.total);
