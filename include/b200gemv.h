@@ -471,7 +471,8 @@ b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* args, b2g_stre
  * page_table[b][pos / page_size]; element (page, row, head, i) is at
  * page * stride_page + row * stride_token + head * stride_head + i, which
  * covers [pages, page_size, heads, dim] and [pages, heads, page_size, dim].
- * The bases are 16-byte aligned and the strides multiples of 16 bytes.
+ * The bases are 16-byte aligned, the strides multiples of 16 bytes, and each
+ * of k and v spans at most 64 GB.
  * E4M3 caches hold value / scale[head] (scale NULL: 1), saturated.
  * New tokens: the rows q_start[b] .. q_start[b + 1] - 1 belong to sequence
  * b, whose last row is its token seq_lens[b] - 1 (seq_lens counts them);

@@ -99,6 +99,7 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
   __shared__ long long sh[8];
   __shared__ float sh_ml[2][16], sh_red[8][16];
   __shared__ int sh_last;
+  __shared__ uint32_t seen_sh[kWarps][kStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   const uint32_t ring = smem_addr(smem) + warp * kStages * kStageBytes;
   float* join = reinterpret_cast<float*>(smem + kWarps * kStages * kStageBytes);
@@ -113,37 +114,44 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
   AttnItem pi = w.find(share.b, at0);
   int pu = pi.u_lo + (int)at0;
   long long left = share.end - share.begin;  // units not yet asked for
-  long long row_at = 0;                      // lanes 0..15: a token's row in the cache, -1: none
+  // Lanes 0..15 (and 16..31 again): a token's row in the cache in units of 16
+  // bytes (a cache spans less than 2^32 of them), and whether it is there.
+  uint32_t row_at = 0;
+  bool row_in = false;
+  const int shift = p.page_shift;
+  constexpr int kPer16 = FP8 ? 16 : 8;  // elements
+  const uint32_t step_token = (uint32_t)(p.c.stride_token / kPer16), step_head = (uint32_t)(p.c.stride_head / kPer16),
+                 step_page = (uint32_t)(p.c.stride_page / kPer16);
   auto look_up = [&]() {
     if (left <= 0) return;
     const int j = pu * kUnit + warp * 16 + (lane & 15);
-    row_at = -1;
+    row_in = false;
     if (j >= pi.lo && j < pi.hi) {
-      const int pg = j / p.c.page_size;
+      const int pg = shift >= 0 ? j >> shift : j / p.c.page_size;
       const int page = page_of(p.b, p.c, pi.b, pg, p.error);
-      if (page >= 0)
-        row_at = page * p.c.stride_page + (long long)(j - pg * p.c.page_size) * p.c.stride_token +
-                 pi.h * p.c.stride_head;
+      row_in = page >= 0;
+      if (row_in) row_at = page * step_page + (j - pg * p.c.page_size) * step_token + pi.h * step_head;
     }
   };
-  uint32_t seen[kStages];  // bit t: the stage's token t is there
   const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
   const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
-  auto copy = [&](uint32_t dst) -> uint32_t {
-    uint32_t mask = 0;
+  // Copies the next unit's tokens; seen_sh: bit t says that token t is there.
+  auto copy = [&](int to) {
     if (left > 0) {
       constexpr int kChunks = kRowBytes / 16, kPerPass = 32 / kChunks;  // tokens a pass of the lanes
       const int c = lane % kChunks;
+      const uint32_t dst = ring + to * kStageBytes;
+      const uint32_t mask = __ballot_sync(0xffffffffu, row_in) & 0xffff;
+      if (lane == 0) seen_sh[warp][to] = mask;
 #pragma unroll
       for (int i = 0; i < 16 / kPerPass; ++i) {
         const int t = i * kPerPass + lane / kChunks;
-        const long long row = __shfl_sync(0xffffffffu, row_at, t);
-        const bool in = row >= 0;
-        const long long off = in ? row * (FP8 ? 1 : 2) + c * 16 : 0;
+        const bool in = mask >> t & 1;
+        const uint32_t row = __shfl_sync(0xffffffffu, row_at, t);  // every lane takes part
+        const unsigned long long off = in ? (unsigned long long)(row + c) * 16 : 0;
         cp_async16_or_zero(dst + chunk_at(t, c), kb + off, in);
         cp_async16_or_zero(dst + kTileBytes + chunk_at(t, c), vb + off, in);
       }
-      mask = __ballot_sync(0xffffffffu, row_at >= 0) & 0xffff;
       --left;
       if (++pu == pi.u_hi && left > 0) {
         w.next(pi);
@@ -151,15 +159,13 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
       }
     }
     cp_async_commit();
-    return mask;
   };
   look_up();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
-    seen[i] = copy(ring + i * kStageBytes);
+    copy(i);
     look_up();
   }
-  seen[kStages - 1] = 0;
 
   // The products.
   at0 = share.at;
@@ -225,6 +231,11 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
     const float scale[2] = {p.a.scale * kLog2e * ks * q_mul[0], p.a.scale * kLog2e * ks * q_mul[1]};
     const int low[2] = {p.a.window > 0 ? row_pos[0] - p.a.window : -1, p.a.window > 0 ? row_pos[1] - p.a.window : -1};
 
+    // Positions of the tile's first and last row: tokens between need no mask.
+    const int first_pos = it.s.ctx + it.tile * kRows / p.group;
+    const int last_low =
+        p.a.window > 0 ? it.s.ctx + (min(it.tile * kRows + kRows, rows) - 1) / p.group - p.a.window : -1;
+
     float o[kNT][4];
 #pragma unroll
     for (int j = 0; j < kNT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -232,20 +243,11 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
 
     for (int n = 0; n < units; ++n) {
       // The stage that was read last is free: ask for the next unit.
-      {
-        const int to = stage == 0 ? kStages - 1 : stage - 1;
-        const uint32_t mask = copy(ring + to * kStageBytes);
-#pragma unroll
-        for (int i = 0; i < kStages; ++i)
-          if (i == to) seen[i] = mask;
-        look_up();
-      }
+      copy(stage == 0 ? kStages - 1 : stage - 1);
+      look_up();
       cp_async_wait<kStages - 1>();
       __syncwarp();
-      uint32_t here = 0;
-#pragma unroll
-      for (int i = 0; i < kStages; ++i)
-        if (i == stage) here = seen[i];
+      const uint32_t here = seen_sh[warp][stage];
       const uint32_t kt = ring + stage * kStageBytes, vt = kt + kTileBytes;
       stage = stage == kStages - 1 ? 0 : stage + 1;
       if (here != 0) {
@@ -280,16 +282,23 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
         }
         // Scores of rows g, g + 8 and tokens 8 nt + 2q, + 1.
         const int j0 = (u0 + n) * kUnit + warp * 16;
-        float mx[2] = {-INFINITY, -INFINITY};
+        float mx[2];
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int t = nt * 8 + 2 * q4 + (e & 1), j = j0 + t, hf = e >> 1;
-            const bool sees = j <= row_pos[hf] && j > low[hf] && (here >> t & 1);
-            s[nt][e] = sees ? (s[nt][e] + s_odd[nt][e]) * scale[hf] : -INFINITY;
-            mx[hf] = fmaxf(mx[hf], s[nt][e]);
-          }
+          for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s_odd[nt][e]) * scale[e >> 1];
+        if (here != 0xffff || j0 + 15 > first_pos || j0 <= last_low) {
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = nt * 8 + 2 * q4 + (e & 1), j = j0 + t, hf = e >> 1;
+              if (!(j <= row_pos[hf] && j > low[hf] && (here >> t & 1))) s[nt][e] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          mx[hf] = fmaxf(fmaxf(s[0][2 * hf], s[0][2 * hf + 1]), fmaxf(s[1][2 * hf], s[1][2 * hf + 1]));
         float al[2];
         bool same = true;
 #pragma unroll

@@ -100,6 +100,7 @@ struct AttnParams {
   b2g_kv_batch b;
   int q_heads, group, bf16;
   int least_units;  // units of work a block at least
+  int page_shift;   // log2 of the page size, -1: no power of two
   int* error;
   int* counters;  // [blocks] zeros, left zero
   void* parts;    // [blocks][2] parts of split items

@@ -63,6 +63,11 @@ b2g_status check_cache(const b2g_kv_cache* c, int32_t act) {
   if (c->num_pages > 1 && c->stride_page < c->head_dim) return B2G_ERR_INVALID;
   if (c->dtype != B2G_DTYPE_FP8_E4M3 && (c->k_scale || c->v_scale)) return B2G_ERR_INVALID;
   if (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4)) return B2G_ERR_INVALID;
+  // The attention counts 16-byte pieces of the cache in 32 bits.
+  const unsigned __int128 span = (unsigned __int128)(c->num_pages - 1) * c->stride_page +
+                                 (unsigned __int128)(c->page_size - 1) * c->stride_token +
+                                 (unsigned __int128)(c->kv_heads - 1) * c->stride_head + c->head_dim;
+  if (span * bytes > (unsigned __int128)1 << 36) return B2G_ERR_UNSUPPORTED;
   return B2G_OK;
 }
 
@@ -318,6 +323,9 @@ b2g_status b2g_attn_enqueue(const b2g_attn* op, const b2g_attn_args* a, const b2
   p.bf16 = op->f.dtype == B2G_DTYPE_BF16;
   p.error = registered_error_word(dev);
   if (!p.error) return B2G_ERR_CUDA;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (c->page_size == 1 << i) p.page_shift = i;
   p.counters = static_cast<int*>(a->workspace);
   p.parts = static_cast<uint8_t*>(a->workspace) + op->off_parts;
   return cuda_status(launch_attention(p, op->num_sms, cu(stream)));
