@@ -399,8 +399,8 @@ b2g_status b2g_stack_enqueue(const b2g_stack* st, int32_t m, void* h, void* act,
  * SiLU and the residual are applied in fp32 and y is rounded once.
  * ------------------------------------------------------------------------ */
 /* Row codes: v = x, or (rmsnorm) v = x * rsqrt(mean(x^2) + rms_eps) * gamma;
- * scale = max(max|v|, 1e-12) / 127 and code = v * (1 / scale) rounded to the
- * nearest integer, ties to even, all in fp32.  A row with a NaN or an infinity gets
+ * scale = max(max|v|, 1e-12) / 127 and code = v / scale rounded to the nearest
+ * integer, ties to even, all in fp32.  A row with a NaN or an infinity gets
  * the scale NaN and zero codes, so that every output of it is NaN.
  * x: [m, ldx] FP16 or BF16, 16-byte aligned, ldx a multiple of 8;
  * codes: [m, ld_codes] int8, 16-byte aligned, ld_codes a multiple of 16 (the

@@ -10,11 +10,29 @@
 namespace b2g {
 namespace {
 
-// v / s rounded to the nearest integer, ties to even, as v * (1 / s): a
-// quotient within 2^-23 of a tie may go the other way.  Adding 1.5 * 2^23
-// leaves the integer in the low bits, in one fused multiply-add a value.
-__device__ __forceinline__ uint32_t code_of(float v, float inv) {
-  return __float_as_uint(__fmaf_rn(v, inv, 12582912.0f)) & 0xff;
+// v / s rounded to the nearest integer, ties to even.  Adding 1.5 * 2^23 to a
+// quotient leaves its integer in the low bits.
+__device__ __forceinline__ uint32_t code_of(float v, float s) {
+  return __float_as_uint(v / s + 12582912.0f) & 0xff;
+}
+// Eight of them, a byte each.  v * (1 / s) is off by at most 2^-22 of it, less
+// than 2^-15: where every product is further than that from a tie its integer
+// is the quotient's, else (one value in 16,000) the quotients are taken.
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s, float inv) {
+  uint32_t w[2] = {0, 0};
+  float off = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = v[e] * inv, r = q + 12582912.0f;
+    off = fmaxf(off, fabsf(q - (r - 12582912.0f)));
+    w[e / 4] |= (__float_as_uint(r) & 0xff) << (8 * (e % 4));
+  }
+  if (off > 0.5f - 0x1p-15f) {
+    w[0] = w[1] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e / 4] |= code_of(v[e], s) << (8 * (e % 4));
+  }
+  return make_uint2(w[0], w[1]);
 }
 __device__ __forceinline__ float scale_of(float amax) {
   return amax <= 3.4028235e38f ? fmaxf(amax, 1e-12f) / 127.0f : __uint_as_float(0x7fffffffu);
@@ -131,22 +149,20 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const I8RowsParams p
     for (int i = 0; i < NC; ++i) {
       const int c = base + i * blockDim.x + threadIdx.x;
       if (c >= chunks) continue;
-      uint32_t w[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e / 4] |= (finite ? code_of(v[i][e], inv) : 0) << (8 * (e % 4));
+      const uint2 w = finite ? codes_of(v[i], s, inv) : make_uint2(0, 0);
       if (8 * c + 8 <= p.k) {
-        *reinterpret_cast<uint2*>(codes + 8 * c) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(codes + 8 * c) = w;
       } else {
-        for (int e = 0; 8 * c + e < p.k; ++e) codes[8 * c + e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
+        for (int e = 0; 8 * c + e < p.k; ++e) codes[8 * c + e] = (int8_t)((e < 4 ? w.x : w.y) >> (8 * (e % 4)));
       }
     }
   }
   if (threadIdx.x == 0) p.scales[row] = s;
 }
 
-// The code of a weight; a channel that is not finite (inv 0) has zero codes.
-__device__ __forceinline__ int8_t channel_code(float v, float inv) {
-  return inv > 0.f ? (int8_t)code_of(v, inv) : (int8_t)0;
+// The code of a weight; a channel that is not finite (s NaN) has zero codes.
+__device__ __forceinline__ int8_t channel_code(float v, float s) {
+  return s == s ? (int8_t)code_of(v, s) : (int8_t)0;
 }
 
 // One-off: 32 output channels a block, both passes over K.
@@ -155,7 +171,7 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
                                                                 int8_t* __restrict__ codes, long long ldc,
                                                                 float* __restrict__ scales) {
   __shared__ float tile[32][33];
-  __shared__ float inv[32];
+  __shared__ float sc[32];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n0 = blockIdx.x * 32;
   float a = 0.f;
@@ -174,7 +190,7 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
     a = 0.f;
     for (int i = 0; i < 32; ++i) a = max_abs(a, tile[i][tx]);
     const float s = scale_of(a);
-    inv[tx] = s == s ? 1.0f / s : 0.f;
+    sc[tx] = s;
     if (n0 + tx < N) scales[n0 + tx] = s;
   }
   __syncthreads();
@@ -182,10 +198,10 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
     if (layout == B2G_LAYOUT_KN) {
       if (k0 + ty < K && n0 + tx < N) tile[ty][tx] = Act<T>::to_float(w[(long long)(k0 + ty) * N + n0 + tx]);
       __syncthreads();
-      if (n0 + ty < N && k0 + tx < K) codes[(n0 + ty) * ldc + k0 + tx] = channel_code(tile[tx][ty], inv[ty]);
+      if (n0 + ty < N && k0 + tx < K) codes[(n0 + ty) * ldc + k0 + tx] = channel_code(tile[tx][ty], sc[ty]);
       __syncthreads();
     } else if (n0 + ty < N && k0 + tx < K) {
-      codes[(n0 + ty) * ldc + k0 + tx] = channel_code(Act<T>::to_float(w[(long long)(n0 + ty) * K + k0 + tx]), inv[ty]);
+      codes[(n0 + ty) * ldc + k0 + tx] = channel_code(Act<T>::to_float(w[(long long)(n0 + ty) * K + k0 + tx]), sc[ty]);
     }
   }
 }
