@@ -1,6 +1,8 @@
 /*
  * b200gemv.h -- C ABI of the B200 (sm_100a) decode-GEMV library for the
- * Llama-3.2-3B MLP projections (gate/up 3072->8192, down 8192->3072, M=1..8).
+ * Llama-3.2-3B MLP projections (gate/up 3072->8192, down 8192->3072, M=1..8),
+ * and of the rest of the layer at any number of rows: 8-bit integer products,
+ * the append to a paged key/value cache and the attention over it.
  *
  * This is the drop-in boundary.  The reference project
  * (sudb97/Llama-3.2-3B-Instruct-gemm-optimization) has no plugin code yet --
@@ -219,7 +221,8 @@ b2g_status b2g_enqueue(const b2g_op* op, int32_t m, const void* x, const void* p
 b2g_status b2g_enqueue_ex(const b2g_op* op, const b2g_enqueue_args* args, b2g_stream_t stream);
 
 /* Reads (and optionally clears) the device error word that kernels set when
- * a bounded wait expires.  Synchronises the current device. */
+ * a bounded wait expires (1 to 5) or a page table names a page that the cache
+ * does not have (6).  Synchronises the current device. */
 b2g_status b2g_device_error(int32_t* code, int32_t clear);
 
 /* ------------------------------------------------------------------------
@@ -537,7 +540,9 @@ b2g_status b2g_kv_append(const b2g_kv_append_args* args, const b2g_kv_cache* cac
  * over the cached tokens j <= pos, and j > pos - window if window > 0.
  * fp32 scores, softmax statistics and sums; the probabilities are rounded to
  * the activations' type for their product with v.  A row that sees nothing
- * gives zeros and the log-sum -infinity. */
+ * gives zeros and the log-sum -infinity.  Cached slots that no row may see
+ * are not read; a NaN or infinity in the v of a token that some rows of a
+ * call see can reach its other rows (0 times it). */
 typedef struct {
   int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads, at most 32 times */
   int32_t head_dim;          /* 64 or 128 */

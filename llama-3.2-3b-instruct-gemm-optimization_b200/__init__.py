@@ -9,7 +9,9 @@ The class names mirror the reference's operator surface:
 ``GemvOp(in_features, out_features, weight_dtype, scale_mode)`` is the planned
 IPluginV3 creator (tensorrt_custom_tactic_kernel_b07f17a4.plan.md:57-58) and
 ``GemvOp.enqueue(x, W, scales) -> y`` replaces ``run_gemv``
-(kernels/gemv_fp8.cu:276-283).
+(kernels/gemv_fp8.cu:276-283).  ``I8Op``, ``PagedCache``, ``kv_append`` and
+``AttnOp`` (together: ``AttentionBlock``) are the rest of a decoder layer at
+any number of rows.
 """
 from __future__ import annotations
 
