@@ -454,8 +454,9 @@ typedef struct {
   void* y;               /* [m, ldy] */
   int64_t ldy;
   void* workspace;       /* b2g_i8_workspace_size bytes, 256-byte aligned, zeroed once by
-                            b2g_i8_workspace_init; calls that can run at the same time
-                            need workspaces of their own */
+                            b2g_i8_workspace_init (again after a call that reported a
+                            device error); this op's only, and calls that can run at the
+                            same time need workspaces of their own */
 } b2g_i8_args;
 b2g_status b2g_i8_create(const b2g_i8_fields* fields, b2g_i8_op** out);
 b2g_status b2g_i8_destroy(b2g_i8_op* op);
@@ -489,7 +490,7 @@ b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* args, b2g_stre
 typedef struct {
   void* k;
   void* v;
-  const float* k_scale; /* [kv_heads], E4M3 only, NULL = 1 */
+  const float* k_scale; /* [kv_heads], positive, E4M3 only, NULL = 1 */
   const float* v_scale;
   int64_t stride_page, stride_token, stride_head; /* elements, the same for k and v */
   int32_t num_pages;
@@ -560,8 +561,9 @@ typedef struct {
   float scale;
   int32_t window; /* 0 = none */
   void* workspace; /* b2g_attn_workspace_size bytes, 256-byte aligned, zeroed once by
-                      b2g_attn_workspace_init; calls that can run at the same time need
-                      workspaces of their own */
+                      b2g_attn_workspace_init (again after a call that reported an expired
+                      wait); calls that can run at the same time need workspaces of their
+                      own */
 } b2g_attn_args;
 b2g_status b2g_attn_create(const b2g_attn_fields* fields, b2g_attn** out);
 b2g_status b2g_attn_destroy(b2g_attn* op);

@@ -537,22 +537,20 @@ def _act_code(t):
     return code
 
 
-def _launch_stream(stream, device, tensors):
-    """The raw stream to launch on, once every tensor is on the current device."""
+def _launch(stream, device):
+    """(index of the current device, which has to be `device`; the raw stream to
+    launch on)."""
     import torch
     if device.type != "cuda":
         raise ValueError(f"tensors on {device}: expected a CUDA device")
     index = device.index
     if index != torch._C._cuda_getDevice():
         raise ValueError(f"tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"tensors on {device} and {t.device}")
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(index)
+        return index, torch._C._cuda_getCurrentRawStream(index)
     if stream.device != device:
         raise ValueError(f"tensors on {device}, a stream of {stream.device}")
-    return stream.cuda_stream
+    return index, stream.cuda_stream
 
 
 def _made(stream, make):
@@ -566,35 +564,42 @@ def _made(stream, make):
         return make()
 
 
-def _matrix(t, dtype, shape, align, what):
+def _refuse(t, index, dtype, shape, what):
+    raise ValueError(f"{what}: expected {list(shape)} {dtype} with contiguous rows on cuda:{index}, got "
+                     f"{tuple(t.shape)} {t.dtype} strides {t.stride()} on {t.device}")
+
+
+def _matrix(t, index, dtype, shape, align, what):
     """The row stride of a matrix with contiguous rows (a single row may carry
     any stride, so it gets an aligned one)."""
-    if t.dtype is dtype and t.shape == shape:
+    if t.dtype is dtype and t.get_device() == index and t.shape == shape:
+        if shape[0] > 1 and t.is_contiguous():
+            return shape[1]
         rows, cols = t.stride()
         if cols == 1 or shape[1] == 1:
             return rows if shape[0] > 1 else -(-shape[1] // align) * align
-    raise ValueError(f"{what}: expected {list(shape)} {dtype} with contiguous rows, got {tuple(t.shape)} {t.dtype} "
-                     f"strides {t.stride()}")
+    _refuse(t, index, dtype, shape, what)
 
 
-def _vector(t, dtype, n, what):
-    if t.dtype is not dtype or t.shape != (n,) or (n > 1 and t.stride() != (1,)):
-        raise ValueError(f"{what}: expected {n} contiguous {dtype}, got {tuple(t.shape)} {t.dtype}")
+def _vector(t, index, dtype, n, what):
+    """The address of n elements."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
+        _refuse(t, index, dtype, (n,), what)
+    return t.data_ptr()
 
 
-def _heads(t, shape, dtype, what):
+def _heads(t, index, dtype, shape, what):
     """(address, row stride, head stride) of [rows, heads, dim]."""
-    if t.dtype is dtype and t.shape == shape:
+    if t.dtype is dtype and t.get_device() == index and t.shape == shape:
         row, head, one = t.stride()
         if one == 1:
             return t.data_ptr(), row, head
-    raise ValueError(f"{what}: expected {list(shape)} {dtype} with a contiguous last axis, got {tuple(t.shape)} "
-                     f"{t.dtype} strides {t.stride()}")
+    _refuse(t, index, dtype, shape, what)
 
 
-def _workspace(ws, need):
-    if ws.nbytes < need or not ws.is_contiguous():
-        raise ValueError(f"the workspace needs {need} contiguous bytes")
+def _workspace(ws, index, need):
+    if ws.get_device() != index or ws.nbytes < need or not ws.is_contiguous():
+        raise ValueError(f"the workspace needs {need} contiguous bytes on cuda:{index}")
     return ws.data_ptr()
 
 
@@ -615,18 +620,16 @@ def quantize_i8_rows(x, gamma=None, rms_eps=None, codes=None, scales=None, strea
     """
     import torch
     m, k = x.shape
-    raw = _launch_stream(stream, x.device, (gamma, codes, scales))
-    ldx = _matrix(x, x.dtype, (m, k), 8, "x")
-    if gamma is not None:
-        _vector(gamma, x.dtype, k, "gamma")
+    index, raw = _launch(stream, x.device)
+    ldx = _matrix(x, index, x.dtype, (m, k), 8, "x")
+    g = 0 if gamma is None else _vector(gamma, index, x.dtype, k, "gamma")
     if codes is None:
         codes = _made(stream, lambda: _codes(m, k, x.device))
     if scales is None:
         scales = _made(stream, lambda: torch.empty(m, dtype=torch.float32, device=x.device))
-    ldc = _matrix(codes, torch.int8, (m, k), 16, "codes")
-    _vector(scales, torch.float32, m, "scales")
-    a = _pack_rows(m, k, _act_code(x), rms_eps is not None, x.data_ptr(), ldx, _address(gamma), rms_eps or 0.0,
-                   codes.data_ptr(), ldc, scales.data_ptr())
+    ldc = _matrix(codes, index, torch.int8, (m, k), 16, "codes")
+    a = _pack_rows(m, k, _act_code(x), rms_eps is not None, x.data_ptr(), ldx, g, rms_eps or 0.0, codes.data_ptr(), ldc,
+                   _vector(scales, index, torch.float32, m, "scales"))
     check(lib().b2g_i8_quantize_rows(a, raw), "b2g_i8_quantize_rows")
     return codes, scales
 
@@ -636,7 +639,7 @@ def quantize_i8_weights(w16, layout="KN", stream=None):
     import torch
     lay = _code(LAYOUT, layout)
     K, N = (w16.shape if lay == 0 else w16.shape[::-1])
-    raw = _launch_stream(stream, w16.device, ())
+    raw = _launch(stream, w16.device)[1]
     if not w16.is_contiguous():
         raise ValueError("w16 must be contiguous")
     codes = _made(stream, lambda: _codes(N, K, w16.device))
@@ -675,7 +678,7 @@ class I8Op:
         return self._ws_bytes
 
     def workspace(self, device="cuda", stream=None):
-        """A zeroed workspace.  Calls that can overlap (other
+        """A zeroed workspace, for this op only.  Calls that can overlap (other
         streams, graphs replayed at the same time) need one each."""
         import torch
         ws = _made(stream, lambda: torch.empty(self._ws_bytes, dtype=torch.uint8, device=device))
@@ -685,40 +688,40 @@ class I8Op:
     def enqueue(self, x, wq, sw, y=None, workspace=None, residual=None, gamma=None, rms_eps: float = 1e-5,
                 stream=None):
         """y of 16-bit rows x [m, K], quantised (and normalised) on the way."""
-        m = x.shape[0]
-        ldx = _matrix(x, self._type, (m, self.K), 8, "x")
-        if gamma is not None:
-            _vector(gamma, self._type, self.K, "gamma")
-        raw = _launch_stream(stream, x.device, (wq, sw, y, workspace, residual, gamma))
-        return self._enqueue(m, x.device, (x.data_ptr(), ldx, _address(gamma), rms_eps, 0, 0, 0), wq, sw, y,
-                             workspace, residual, stream, raw)
+        device, m = x.device, x.shape[0]
+        index, raw = _launch(stream, device)
+        ldx = _matrix(x, index, self._type, (m, self.K), 8, "x")
+        g = 0 if gamma is None else _vector(gamma, index, self._type, self.K, "gamma")
+        return self._enqueue(m, device, index, (x.data_ptr(), ldx, g, rms_eps, 0, 0, 0), wq, sw, y, workspace, residual,
+                             stream, raw)
 
     def enqueue_codes(self, xq, sx, wq, sw, y=None, workspace=None, residual=None, stream=None):
         """y of rows that quantize_i8_rows has quantised (one quantisation, several products)."""
         import torch
-        m = xq.shape[0]
-        ldx = _matrix(xq, torch.int8, (m, self.K), 16, "xq")
-        _vector(sx, torch.float32, m, "sx")
-        raw = _launch_stream(stream, xq.device, (sx, wq, sw, y, workspace, residual))
-        return self._enqueue(m, xq.device, (0, 0, 0, 0.0, xq.data_ptr(), ldx, sx.data_ptr()), wq, sw, y, workspace,
-                             residual, stream, raw)
+        device, m = xq.device, xq.shape[0]
+        index, raw = _launch(stream, device)
+        ldx = _matrix(xq, index, torch.int8, (m, self.K), 16, "xq")
+        return self._enqueue(m, device, index, (0, 0, 0, 0.0, xq.data_ptr(), ldx, _vector(sx, index, torch.float32, m, "sx")),
+                             wq, sw, y, workspace, residual, stream, raw)
 
-    def _enqueue(self, m, device, x_args, wq, sw, y, workspace, residual, stream, raw):
+    def _enqueue(self, m, device, index, x_args, wq, sw, y, workspace, residual, stream, raw):
         import torch
-        rows = self.planes * self.N
-        ldw = _matrix(wq, torch.int8, (rows, self.K), 16, "wq")
-        _vector(sw, torch.float32, rows, "sw")
-        ldr = 0 if residual is None else _matrix(residual, self._type, (m, self.N), 1, "residual")
+        rows, shape = self.planes * self.N, (m, self.N)
+        ldw = _matrix(wq, index, torch.int8, (rows, self.K), 16, "wq")
+        scales = _vector(sw, index, torch.float32, rows, "sw")
+        res, ldr = 0, 0
+        if residual is not None:
+            res, ldr = residual.data_ptr(), _matrix(residual, index, self._type, shape, 1, "residual")
         if y is None:
-            y = _made(stream, lambda: torch.empty((m, self.N), dtype=self._type, device=device))
+            y = _made(stream, lambda: torch.empty(shape, dtype=self._type, device=device))
             ldy = self.N
         else:
-            ldy = _matrix(y, self._type, (m, self.N), 1, "y")
+            ldy = _matrix(y, index, self._type, shape, 1, "y")
         if workspace is None:
             workspace = self.workspace(device, stream)
-        a = _pack_i8(m, *x_args, wq.data_ptr(), ldw, sw.data_ptr(), _address(residual), ldr, y.data_ptr(), ldy,
-                     _workspace(workspace, self._ws_bytes))
-        status = lib().b2g_i8_enqueue(self.h, a, raw)
+        a = _pack_i8(m, *x_args, wq.data_ptr(), ldw, scales, res, ldr, y.data_ptr(), ldy,
+                     _workspace(workspace, index, self._ws_bytes))
+        status = _lib.b2g_i8_enqueue(self.h, a, raw)
         if status:
             check(status, "b2g_i8_enqueue")
         return y
@@ -741,10 +744,10 @@ class PagedCache:
         tok, head = (1, 2) if layout == "NHD" else (2, 1)
         for s in (k_scale, v_scale):
             if s is not None:
-                _vector(s, torch.float32, k.shape[head], "k_scale, v_scale")
-        if any(t is not None and t.device != k.device for t in (v, k_scale, v_scale)):
+                _vector(s, k.get_device(), torch.float32, k.shape[head], "k_scale, v_scale")
+        if v.device != k.device:
             raise ValueError("the cache's tensors are on different devices")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.k, self.v, self.k_scale, self.v_scale, self.index = k, v, k_scale, v_scale, k.get_device()
         self.page_size, self.kv_heads, self.head_dim, self.dtype = k.shape[tok], k.shape[head], k.shape[3], code
         # The tensors are held above, so their addresses stay theirs.
         self.packed = _pack_cache(k.data_ptr(), v.data_ptr(), _address(k_scale), _address(v_scale), k.stride(0),
@@ -752,17 +755,22 @@ class PagedCache:
                                   self.head_dim, code)
 
 
-def _batch(rows, q_start, seq_lens, page_table, max_q):
+def _batch(index, rows, q_start, seq_lens, page_table, max_q):
     import torch
     batch = seq_lens.shape[0]
-    _vector(q_start, torch.int32, batch + 1, "q_start")
-    _vector(seq_lens, torch.int32, batch, "seq_lens")
     if page_table.dim() != 2:
         raise ValueError("page_table: expected [batch, pages]")
     pages = page_table.shape[1]
-    ld = _matrix(page_table, torch.int32, (batch, pages), 1, "page_table")
-    return _pack_batch(batch, rows, rows if max_q is None else max_q, pages, ld, q_start.data_ptr(),
-                       seq_lens.data_ptr(), page_table.data_ptr())
+    ld = _matrix(page_table, index, torch.int32, (batch, pages), 1, "page_table")
+    return _pack_batch(batch, rows, rows if max_q is None else max_q, pages, ld,
+                       _vector(q_start, index, torch.int32, batch + 1, "q_start"),
+                       _vector(seq_lens, index, torch.int32, batch, "seq_lens"), page_table.data_ptr())
+
+
+def _cache(cache, index):
+    if cache.index != index:
+        raise ValueError(f"the cache is on cuda:{cache.index}, the call's tensors on cuda:{index}")
+    return cache.packed
 
 
 def kv_append(k, v, cache, q_start, seq_lens, page_table, q=None, q_out=None, inv_freq=None,
@@ -776,21 +784,21 @@ def kv_append(k, v, cache, q_start, seq_lens, page_table, q=None, q_out=None, in
     """
     import torch
     rows, dim, t = k.shape[0], cache.head_dim, k.dtype
-    raw = _launch_stream(stream, k.device, (v, cache.k, q_start, seq_lens, page_table, q, q_out, inv_freq))
+    index, raw = _launch(stream, k.device)
     shape = (rows, cache.kv_heads, dim)
-    heads, qq, qo, n_freq = 0, (0, 0, 0), (0, 0, 0), 0
+    heads, qq, qo, n_freq, freq = 0, (0, 0, 0), (0, 0, 0), 0, 0
     if q is not None:
         heads = q.shape[1]
-        qq = _heads(q, (rows, heads, dim), t, "q")
-        qo = qq if q_out is None else _heads(q_out, (rows, heads, dim), t, "q_out")
+        qq = _heads(q, index, t, (rows, heads, dim), "q")
+        qo = qq if q_out is None else _heads(q_out, index, t, (rows, heads, dim), "q_out")
     elif q_out is not None:
         raise ValueError("q_out without q")
     if inv_freq is not None:
         n_freq = inv_freq.shape[0]
-        _vector(inv_freq, torch.float32, n_freq, "inv_freq")
-    a = _pack_append(_act_code(k), heads, n_freq, interleaved, _address(inv_freq), *_heads(k, shape, t, "k"),
-                     *_heads(v, shape, t, "v"), *qq, *qo)
-    status = lib().b2g_kv_append(a, cache.packed, _batch(rows, q_start, seq_lens, page_table, 1), raw)
+        freq = _vector(inv_freq, index, torch.float32, n_freq, "inv_freq")
+    a = _pack_append(_act_code(k), heads, n_freq, interleaved, freq, *_heads(k, index, t, shape, "k"),
+                     *_heads(v, index, t, shape, "v"), *qq, *qo)
+    status = lib().b2g_kv_append(a, _cache(cache, index), _batch(index, rows, q_start, seq_lens, page_table, 1), raw)
     if status:
         check(status, "b2g_kv_append")
     return q if q_out is None else q_out
@@ -839,22 +847,26 @@ class AttnOp:
         """
         import torch
         rows, device = q.shape[0], q.device
-        raw = _launch_stream(stream, device, (cache.k, q_start, seq_lens, page_table, out, lse, workspace))
+        index, raw = _launch(stream, device)
         shape = (rows, self.q_heads, self.head_dim)
-        qq = _heads(q, shape, self._type, "q")
+        qq = _heads(q, index, self._type, shape, "q")
         if out is None:
             out = _made(stream, lambda: torch.empty(shape, dtype=self._type, device=device))
             oo = (out.data_ptr(), self.q_heads * self.head_dim, self.head_dim)
         else:
-            oo = _heads(out, shape, self._type, "out")
-        if lse is not None and (lse.dtype is not torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
-            raise ValueError(f"lse: expected [{rows}, {self.q_heads}] contiguous float32")
+            oo = _heads(out, index, self._type, shape, "out")
+        sums = 0
+        if lse is not None:
+            if lse.dtype is not torch.float32 or lse.get_device() != index or lse.shape != shape[:2] or \
+                    not lse.is_contiguous():
+                _refuse(lse, index, torch.float32, shape[:2], "lse")
+            sums = lse.data_ptr()
         if workspace is None:
             workspace = self.workspace(device, stream)
-        a = _pack_attn(*qq, *oo, _address(lse), self.head_dim ** -0.5 if scale is None else scale, window,
-                       _workspace(workspace, self._ws_bytes))
-        status = lib().b2g_attn_enqueue(self.h, a, cache.packed, _batch(rows, q_start, seq_lens, page_table, max_q),
-                                        raw)
+        a = _pack_attn(*qq, *oo, sums, self.head_dim ** -0.5 if scale is None else scale, window,
+                       _workspace(workspace, index, self._ws_bytes))
+        status = _lib.b2g_attn_enqueue(self.h, a, _cache(cache, index),
+                                       _batch(index, rows, q_start, seq_lens, page_table, max_q), raw)
         if status:
             check(status, "b2g_attn_enqueue")
         return out
@@ -892,6 +904,8 @@ class AttentionBlock:
 
     def enqueue(self, h, cache, q_start, seq_lens, page_table, workspace, max_q=None, window: int = 0, stream=None):
         m = h.shape[0]
+        if m > self._rows.shape[0]:
+            raise ValueError(f"{m} rows: the block was made for {self._rows.shape[0]}")
         rows = self._rows[:m]
         self.qkv.enqueue(h, *self.wqkv, y=rows.view(m, -1), workspace=workspace[0], gamma=self.gamma,
                          rms_eps=self.rms_eps, stream=stream)

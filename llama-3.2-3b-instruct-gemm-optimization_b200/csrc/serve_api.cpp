@@ -305,6 +305,8 @@ b2g_status b2g_attn_enqueue(const b2g_attn* op, const b2g_attn_args* a, const b2
   if (c->dtype != op->f.cache_dtype || c->kv_heads != op->f.kv_heads || c->head_dim != op->f.head_dim)
     return B2G_ERR_INVALID;
   if (b->batch > op->f.max_batch) return B2G_ERR_INVALID;
+  // Rows are counted per k/v head in 32 bits.
+  if ((int64_t)b->rows * (op->f.q_heads / op->f.kv_heads) > (1 << 30)) return B2G_ERR_UNSUPPORTED;
   const int dim = op->f.head_dim, heads = op->f.q_heads;
   if (!heads16(a->q, a->stride_q, a->stride_q_head, heads, dim, b->rows)) return B2G_ERR_INVALID;
   if (!heads16(a->out, a->stride_o, a->stride_o_head, heads, dim, b->rows)) return B2G_ERR_INVALID;
@@ -316,6 +318,7 @@ b2g_status b2g_attn_enqueue(const b2g_attn* op, const b2g_attn_args* a, const b2
   if (dev != op->device) return B2G_ERR_INVALID;
   AttnParams p = {};
   p.a = *a;
+  if (p.a.window > (1 << 30)) p.a.window = 1 << 30;  // more than a cache holds
   p.c = *c;
   p.b = *b;
   p.q_heads = heads;

@@ -152,7 +152,9 @@ def test_attn_fields(b2g, no_gpu, f, want):
                              dict(workspace=A + 64))]
                          + [({}, c, {}, w) for c, w in BAD_CACHE] + [({}, {}, b, w) for b, w in BAD_BATCH]
                          + [({}, dict(kv_heads=1), {}, INVALID), ({}, dict(head_dim=64), {}, INVALID),
-                            ({}, dict(dtype=1), {}, INVALID), ({}, {}, dict(batch=3), INVALID)])
+                            ({}, dict(dtype=1), {}, INVALID), ({}, {}, dict(batch=3), INVALID),
+                            ({}, {}, dict(rows=1 << 30), UNSUPPORTED), ({}, dict(num_pages=1 << 24), {}, UNSUPPORTED),
+                            (dict(window=2 ** 31 - 1), {}, {}, CUDA), (dict(window=5), {}, {}, CUDA)])
 def test_attn_arguments(b2g, no_gpu, args, cache, batch, want):
     op = b2g.AttnOp(4, 2, 128, max_batch=2)
     call = lambda a, c, b: b2g.lib().b2g_attn_enqueue(  # noqa: E731
