@@ -43,27 +43,32 @@ __device__ __forceinline__ float max_abs(float a, float v) {
   return __uint_as_float(max(__float_as_uint(a), __float_as_uint(v) & 0x7fffffffu));
 }
 
-// Elements 8c .. 8c + 7 of a row of k (zeros behind its end).
+// Elements 8c .. 8c + 7 of a row of k, as they are (zeros behind its end).
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int c, int k, float (&f)[8]) {
-  if (8 * c + 8 <= k) {
-    const uint4 v = *reinterpret_cast<const uint4*>(row + 8 * c);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ uint4 load8(const T* row, int c, int k) {
+  if (8 * c + 8 <= k) return *reinterpret_cast<const uint4*>(row + 8 * c);
+  uint32_t w[4] = {0, 0, 0, 0};
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = Act<T>::unpack(w[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
-  } else {
+  for (int i = 0; i < 8; ++i)
+    if (8 * c + i < k) w[i / 2] |= (uint32_t)h[8 * c + i] << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = 8 * c + i < k ? Act<T>::to_float(row[8 * c + i]) : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = Act<T>::unpack(w[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
   }
 }
 
-// One block a row.  A thread keeps up to 32 elements (four 16-byte loads) in
-// registers, so a row of up to 32 x threads elements is read once; a longer
-// one is read again for each pass.
+// One block a row.  A thread keeps up to 32 elements (four 16-byte loads) as
+// they come, so a row of up to 32 x threads elements is read once (a longer
+// one again for each pass) and six blocks an SM fit; each pass widens and
+// normalises them again, to the same bits.
 template <typename T, bool RMS>
 __global__ void __launch_bounds__(512) quantize_rows_kernel(const I8RowsParams p) {
   constexpr int NC = 4;
@@ -76,29 +81,29 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const I8RowsParams p
   const bool resident = chunks <= per_pass;
   pdl_wait();
   pdl_launch_dependents();  // behind the wait: the launch after this one may read weights at once
-  float v[NC][8];
+  uint4 raw[NC];
   auto load = [&](int base) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = base + i * blockDim.x + threadIdx.x;
-      if (c < chunks) {
-        load8(x, c, p.k, v[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-      }
+      raw[i] = c < chunks ? load8(x, c, p.k) : make_uint4(0, 0, 0, 0);
     }
   };
   float r = 1.0f;
-  auto normalise = [&](int base) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
+  // Chunk i of the pass at `base`, normalised.
+  auto values = [&](int base, int i, float (&v)[8]) {
+    unpack8<T>(raw[i], v);
+    if constexpr (RMS) {
       const int c = base + i * blockDim.x + threadIdx.x;
-      if (c >= chunks) continue;
-      float g[8];
-      if (gamma) load8(gamma, c, p.k, g);
+      if (gamma && c < chunks) {
+        float g[8];
+        unpack8<T>(load8(gamma, c, p.k), g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = gamma ? v[i][e] * r * g[e] : v[i][e] * r;
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * r * g[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= r;
+      }
     }
   };
   load(0);
@@ -107,9 +112,12 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const I8RowsParams p
     for (int base = 0; base < chunks; base += per_pass) {
       if (base) load(base);
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
+      for (int i = 0; i < NC; ++i) {
+        float v[8];
+        unpack8<T>(raw[i], v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
+        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+      }
     }
     for (int off = 16; off; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     if (lane == 0) red[0][warp] = ss;
@@ -118,18 +126,17 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const I8RowsParams p
     for (int off = 16; off; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
     r = rsqrtf(ss / (float)p.k + p.eps);
     if (!resident) load(0);
-    normalise(0);
   }
   float a = 0.f;
   for (int base = 0; base < chunks; base += per_pass) {
-    if (base) {
-      load(base);
-      if constexpr (RMS) normalise(base);
+    if (base) load(base);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      float v[8];
+      values(base, i, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = max_abs(a, v[e]);
     }
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) a = max_abs(a, v[i][e]);
   }
   for (int off = 16; off; off >>= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, off));
   if (lane == 0) red[1][warp] = a;
@@ -141,15 +148,14 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const I8RowsParams p
   const float inv = 1.0f / s;
   int8_t* codes = p.codes + row * p.ldc;
   for (int base = 0; base < chunks; base += per_pass) {
-    if (!resident) {
-      load(base);
-      if constexpr (RMS) normalise(base);
-    }
+    if (!resident) load(base);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = base + i * blockDim.x + threadIdx.x;
       if (c >= chunks) continue;
-      const uint2 w = finite ? codes_of(v[i], s, inv) : make_uint2(0, 0);
+      float v[8];
+      values(base, i, v);
+      const uint2 w = finite ? codes_of(v, s, inv) : make_uint2(0, 0);
       if (8 * c + 8 <= p.k) {
         *reinterpret_cast<uint2*>(codes + 8 * c) = w;
       } else {

@@ -156,6 +156,35 @@ def test_bf16_rows_out_of_fp16_range_over_8bit_cache(b2g, cuda):
     check(b2g, [40], [130], 4, 2, 128, 16, "bf16", "e4m3", q=q, scale=1e7)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("cache", ["fp16", "e4m3"])
+def test_offsets_beyond_32_bits(b2g, cuda, new, cache):
+    """Two pages 34 GB apart: beyond 2^32 elements, and 2^31 pieces of 16 bytes."""
+    d, page, total = 128, 16, 24
+    size = 1 if cache == "e4m3" else 2
+    gap = (34 << 30) // size  # elements
+    buf = torch.empty(gap * size + (1 << 20), dtype=torch.uint8, device="cuda").view(TYPES[cache])
+    shape, strides = (2, page, 2, d), (gap, 4 * d, d, 1)
+    k, v = buf.as_strided(shape, strides), buf.as_strided(shape, strides, 2 * d)
+    kv = b2g.PagedCache(k, v)
+    starts, lens, table = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, total], [total], [[1, 0]]))
+    x = torch.randn(total, 2, 2, d, device="cuda").half()
+    b2g.kv_append(x[:, 0], x[:, 1], kv, starts, lens, table)
+    q = rand_q(new, 4, d, "fp16")  # 40 new rows: the first 16 lie before the start
+    starts = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+    op = b2g.AttnOp(4, 2, d, 1, cache_dtype=cache)
+    out = op.enqueue(q, kv, starts, lens, table, max_q=new)
+    torch.cuda.synchronize()
+    assert b2g.device_error() == 0
+    small = [torch.stack([c[0], c[1]]).contiguous() for c in (k.view(torch.uint8) if size == 1 else k,
+                                                             v.view(torch.uint8) if size == 1 else v)]
+    small = [c.view(TYPES[cache]) for c in small]
+    want, _, bound = attention(q, *small, [new], [total], table)
+    assert bool(((out.double() - want).abs() <= bound).all())
+    del buf, k, v, kv
+    torch.cuda.empty_cache()
+
+
 def test_strided_q_and_out(b2g, cuda):
     """q and out inside wider rows, as a fused projection leaves them."""
     hq, hkv, d, n = 4, 2, 128, 5
