@@ -14,7 +14,9 @@ cudaError_t launch_rows(AttnParams p, int num_sms, cudaStream_t stream) {
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, FP8, D>), K::kSmem, &allowed);
   if (e != cudaSuccess) return e;
-  p.least_units = 4;
+  // Two units a block at least: one sequence of 1000 tokens 11.2 us (13.2 with
+  // four), of 4001 15.8 (16.5).
+  p.least_units = 2;
   return launch_after(attn_rows_kernel<T, FP8, D>, dim3(K::kBlocks * num_sms), dim3(128), K::kSmem, 1, stream, p);
 }
 
