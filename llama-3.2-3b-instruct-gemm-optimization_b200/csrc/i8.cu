@@ -227,11 +227,12 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
 // one: 240 clocks an MMA of 128 x 256 where the tensor cores need 128), but
 // fills tensor memory with one accumulator, drained by eight warps between
 // tiles.
-// Work is cut in one of three ways.  Whole tiles, where they fill the SMs.  A
+// Work is cut in one of three ways (i8_plan).  Whole tiles, in turn.  A
 // cluster of 2, 4 or 8 CTAs a tile, where that many fit: each takes a part of K
 // and leaves its int32 sums in its shared memory, and each finishes a part of
 // the columns from everybody's (one token by 8192 x 4096: 13 us, 18.6 through
-// global memory).  Else equal ranges of k blocks ("units"): a range's tiles at
+// global memory).  For a long K and very few tiles equal ranges of k blocks
+// ("units"; 30 x 300 x 8000: 7.9 us, clusters of eight 10.9): a range's tiles at
 // its two ends are shared with other CTAs, which all add their int32 sums into
 // the workspace (integers: the order does not matter); the last to arrive
 // finishes the tile and leaves zeros behind.
@@ -653,14 +654,6 @@ bool encode_rows(CUtensorMap* map, const void* base, long long rows, long long c
 }
 
 int up32(int n) { return (n + 31) / 32 * 32; }
-// Tokens of a tile for m rows: the fewest tiles of at most 256 / planes
-// columns, evened out.
-int i8_bn(int m, int planes) {
-  const int most = 256 / planes;
-  const int tiles = (m + most - 1) / most;
-  return up32((m + tiles - 1) / tiles);
-}
-
 template <typename T, int PLANES, bool GATE, bool DEEP>
 cudaError_t launch_product(const I8Tc& t, int grid, int smem, cudaStream_t stream) {
   static std::atomic<uint64_t> allowed{0};  // devices whose limit is set
@@ -680,6 +673,55 @@ cudaError_t launch_typed(const I8Tc& t, bool deep, int grid, int smem, cudaStrea
 }
 
 int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// How a product is cut: columns of a tile, one of the ways above.
+struct I8Plan {
+  int bn = 0, cluster = 1;
+  bool deep = false, whole = true;
+};
+
+// The cut with the least estimated time.  The terms, in ns, were fitted to 90
+// products of 1..8000 tokens, each timed under every cut (the choice is 1.1% off
+// the best of them on average; choosing by how full the last wave is was 34% off):
+// a k block takes 400 a plane (540 a deep one), or what L2 delivers to all CTAs at
+// 14.5 bytes a ns; an epilogue 20 a column (26 next to the next tile's loads, 24 deep).
+I8Plan i8_plan(int m, int n, int k, int planes, int num_sms) {
+  const int kb = div_up(k, kKBlock), ch = div_up(n, kChTile);
+  // Clusters of 4 and 8 that the GPCs of 148 SMs hold: 33 and 15.
+  const int fit[9] = {0, 0, num_sms / 2, 0, num_sms * 9 / 40, 0, 0, 0, (num_sms + 2) / 10};
+  I8Plan best;
+  double least = 1e30;
+  const auto take = [&](double ns, int bn, int cluster, bool deep, bool whole) {
+    if (ns >= least) return;
+    least = ns;
+    best.bn = bn, best.cluster = cluster, best.deep = deep, best.whole = whole;
+  };
+  const auto block_ns = [&](double alone, int ctas, int rows) {
+    return std::max(alone, std::min(ctas, num_sms) * (rows * (double)kKBlock) / 14500);
+  };
+  // Tiles of a quarter of the most columns at least: smaller ones never won.
+  const int most = std::min(up32(m), 256 / planes);
+  for (int bn = most; bn >= std::max(32, most / 4); bn -= 32) {
+    const int tiles = div_up(m, bn) * ch, rows = planes * kChTile + bn;
+    const double loop = kb * block_ns(400 * planes, tiles, rows), tail = 20.0 * bn;
+    take(loop + tail + (div_up(tiles, num_sms) - 1) * std::max(loop, 26.0 * bn), bn, 1, false, true);
+    for (int c = 2; c <= 8 && c <= kb; c *= 2)
+      if (tiles <= fit[c])
+        take(div_up(kb, c) * block_ns(400 * planes, tiles * c, rows) + (c == 2 ? 700 : c == 4 ? 1800 : 4100) +
+                 28.0 * bn * planes, bn, c, false, true);
+    if (bn == most) {  // shared ranges: atomics for each valid column, and two waits
+      const long long units = (long long)tiles * kb;
+      take(3300 + div_up(units, std::min<long long>(units, num_sms)) * 1050.0 * planes +
+               63.0 * std::min(bn, m) * planes, bn, 1, false, false);
+    }
+  }
+  const int deep_most = std::min(up32(m), 256), deep_ch = planes == 2 ? ch : div_up(n, 2 * kChTile);
+  for (int bn = deep_most; bn >= std::max(32, deep_most / 2); bn -= 16) {
+    const int tiles = div_up(m, bn) * deep_ch;
+    take(div_up(tiles, num_sms) * (kb * block_ns(540, tiles, 2 * kChTile + bn) + 24.0 * bn), bn, 1, true, true);
+  }
+  return best;
+}
 
 }  // namespace
 
@@ -712,29 +754,13 @@ size_t i8_partial_bytes(int max_m, int planes, int num_sms) {
 
 cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int* partials, int* error,
                               bool after_quantiser, cudaStream_t stream) {
+  const I8Plan plan = i8_plan(p.m, p.n, p.k, p.planes, num_sms);
+  const bool deep = plan.deep;
   I8Tc t;
   t.p = p;
-  t.bn = i8_bn(p.m, p.planes);
+  t.bn = plan.bn;
   t.tok_tiles = div_up(p.m, t.bn);
-  t.tiles = t.tok_tiles * div_up(p.n, kChTile);
-  // Whole tiles take (waves of tiles) x (columns of a tile's products).  A deep
-  // tile has twice a narrow one's rows (or, gate||up, the narrow one's planes
-  // and up to twice its columns), at 0.7 of the time for each product; its
-  // columns (a multiple of 16) are chosen for the fewest waves x columns.
-  const int deep_ch = div_up(p.n, p.planes == 2 ? kChTile : 2 * kChTile);
-  long long deep_cost = 0;
-  int deep_bn = 0;
-  for (int bn = 144; bn <= 256; bn += 16) {
-    const long long cost = (long long)div_up((long long)deep_ch * div_up(p.m, bn), num_sms) * bn;
-    if (!deep_bn || cost <= deep_cost) deep_cost = cost, deep_bn = bn;
-  }
-  const long long narrow_cost = (long long)div_up(t.tiles, num_sms) * t.bn;
-  const bool deep = deep_cost * (p.planes == 2 ? 10 : 20) * 7 < narrow_cost * 100 && t.tiles >= num_sms;
-  if (deep) {
-    t.bn = deep_bn;
-    t.tok_tiles = div_up(p.m, t.bn);
-    t.tiles = t.tok_tiles * deep_ch;
-  }
+  t.tiles = t.tok_tiles * div_up(p.n, deep && p.planes == 1 ? 2 * kChTile : kChTile);
   const int stage_tiles = deep ? 2 : p.planes;
   const int stage_bytes = (stage_tiles * kChTile + t.bn) * kKBlock;
   t.stages = std::min(kI8MaxStages, (kI8SmemBytes - 1024) / stage_bytes);
@@ -751,16 +777,10 @@ cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int
   t.counters = counters;
   t.partials = partials;
   t.error = error;
-  // Whole tiles where the last wave leaves at most a tenth of the SMs' time idle.
-  const int waves = div_up(t.tiles, num_sms);
-  t.whole = deep || t.tiles * 10LL >= (long long)waves * num_sms * 9;
-  int grid = (int)std::min<long long>(t.whole ? t.tiles : t.units, num_sms);
-  // A cluster a tile where at least two CTAs fit for every tile (a GPC holds
-  // 16 SMs or more, so sizes up to 8 pack without much loss).
-  t.cluster = 1;
-  while (!t.whole && t.cluster < 8 && t.tiles * t.cluster * 2 <= num_sms * 9 / 10 && t.cluster * 2 <= t.kb)
-    t.cluster *= 2;
-  if (t.cluster > 1) grid = t.tiles * t.cluster;
+  t.whole = plan.whole;
+  t.cluster = plan.cluster;
+  const int grid = t.cluster > 1 ? t.tiles * t.cluster
+                                 : (int)std::min<long long>(t.whole ? t.tiles : t.units, num_sms);
   t.after_quantiser = after_quantiser;
   if (!encode_rows(&t.mw, p.w, (long long)p.planes * p.n, p.k, p.ldw, kChTile) ||
       !encode_rows(&t.mx, p.x, p.m, p.k, p.ldx, t.bn))

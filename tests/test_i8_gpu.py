@@ -61,7 +61,9 @@ def check_product(b2g, m, n, k, dtype="fp16", fuse=0, seed=3, ldx=None, op=None,
 SHAPES = [(1, 1, 1), (1, 128, 128), (2, 17, 40), (5, 100, 1000), (32, 128, 256), (33, 129, 129), (1, 4096, 2048),
           (8, 1024, 8192), (64, 2048, 512), (100, 8192, 256), (127, 300, 4096), (256, 19000, 128), (257, 513, 77),
           (300, 9600, 1024), (517, 1000, 640), (1, 20000, 64), (700, 5000, 300),
-          (1000, 6000, 700), (1500, 5000, 333), (2049, 4100, 130)]
+          (1000, 6000, 700), (1500, 5000, 333), (2049, 4100, 130),
+          (30, 300, 8000), (34, 221, 7296), (512, 1024, 1500), (146, 272, 7184), (281, 1712, 1500), (2997, 1121, 136),
+          (61, 6288, 448), (1026, 2241, 640)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
