@@ -764,10 +764,11 @@ cudaError_t launch_i8_product(const I8Params& p, int num_sms, int* counters, int
   const int stage_tiles = deep ? 2 : p.planes;
   const int stage_bytes = (stage_tiles * kChTile + t.bn) * kKBlock;
   t.stages = std::min(kI8MaxStages, (kI8SmemBytes - 1024) / stage_bytes);
-  // Narrow tiles leave room for a second CTA, the next launch's: it sets
-  // itself up while this one runs (12.9 us a product of 1 x 8192 x 4096
-  // instead of 14.1), and 100 KB in flight still hide the latency.
-  if (t.bn * stage_tiles <= 64) t.stages = std::min(t.stages, 100 * 1024 / stage_bytes);
+  // Narrow tiles of one plane leave room for a second CTA, the next launch's: it
+  // sets itself up while this one runs (12.9 us a product of 1 x 8192 x 4096
+  // instead of 14.1), and 100 KB in flight still hide the latency.  Two planes
+  // need the bytes (gate||up of 8 x 8192 x 4096: 16.3 us, 19.9 with 74 KB).
+  if (t.bn <= 64 && stage_tiles == 1) t.stages = std::min(t.stages, 100 * 1024 / stage_bytes);
   t.kb = div_up(p.k, kKBlock);
   t.units = (long long)t.tiles * t.kb;
   t.acc_cols = deep ? 256 : t.bn;
