@@ -9,6 +9,9 @@
 // m16n8k16 fragments.  At the end of an item the warps' parts are joined in
 // shared memory, and the blocks' parts of a split item by the last block to
 // arrive, always in the same order.
+// 64 sequences of up to 8192 tokens, 32 heads on 8, bf16: 209 us, 0.94 of a
+// copy's rate.  Two of 131072 over an 8-bit cache, 4 tokens each: 130 us, 0.63
+// (widening the codes takes the issue slots).
 #pragma once
 #include <type_traits>
 

@@ -23,6 +23,10 @@
 // one buffer of 128 columns a unit took 4650 clocks, 1800 of them from a P to
 // the next S).  A tile's S(u + 2) is issued behind its O += P(u) V(u) into the
 // same buffer and one commit covers both.
+// Three chunks of up to 2048 tokens at up to 6000, 32 heads on 8, bf16: 388 us in
+// a short run, 0.91 PFLOP/s (436 in a long one at the power limit);
+// the softmax warps take 2000 clocks for 64 columns of both tiles, of which
+// the exponentials are 1024.
 // Every wait is bounded; after one has run out its thread goes through the
 // remaining steps without waiting, so that barriers still meet.
 #pragma once
