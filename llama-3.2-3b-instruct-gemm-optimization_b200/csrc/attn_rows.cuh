@@ -109,7 +109,7 @@ __device__ void RowsKernel<T, FP8, D>::run(const AttnParams& p) {
   pdl_wait();
   pdl_launch_dependents();
   const Work w(p);
-  const AttnShare share = attn_share(w, p.least_units, sh);
+  const AttnShare share = attn_share<false>(w, p.least_units, sh);
   if (share.begin >= share.end) return;
 
   // The stream of units: where the copies are, ahead of the products.

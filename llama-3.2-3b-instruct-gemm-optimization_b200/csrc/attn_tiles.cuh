@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(512, 1) attn_tiles_kernel(const __grid_constan
   pdl_wait();
   pdl_launch_dependents();
   const typename K::Work w(p);
-  const AttnShare share = attn_share(w, p.least_units, s.share);  // synchronises the block
+  const AttnShare share = attn_share<true>(w, p.least_units, s.share);  // synchronises the block
   tc_fence_after();
   if (warp < 8) {
     K::softmax(p, s, share, warp >> 2);

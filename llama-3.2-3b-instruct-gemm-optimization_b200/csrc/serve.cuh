@@ -165,8 +165,9 @@ struct AttnWork {
     it.u_lo = it.lo / UNIT;
     it.u_hi = max((it.hi + UNIT - 1) / UNIT, it.u_lo + 1);
   }
-  // Units of a sequence's items.
-  __host__ __device__ __forceinline__ long long units(int b) const {
+  // Units of a sequence's items; *longer is set if they are more than four on
+  // average.
+  __host__ __device__ __forceinline__ long long units(int b, bool* longer = nullptr) const {
     AttnItem it;
     it.s = seq_span(p.b, b);
     long long n = 0;
@@ -175,6 +176,7 @@ struct AttnWork {
       range(it);
       n += it.u_hi - it.u_lo;
     }
+    if (longer) *longer |= n > 4LL * nt;
     return n * p.c.kv_heads;
   }
   // The item that holds unit `at` of sequence b; `at` becomes the unit's
@@ -226,14 +228,17 @@ __host__ __device__ __forceinline__ long long attn_begin(const AttnShare& s, int
 
 // Sums the list (all threads; sh: blockDim.x + 1 words) and finds the block's
 // range.  At least `least` units a block, so that short work is not cut finer
-// than the joining of its pieces is worth.
-template <typename Work>
+// than the joining of its pieces is worth; BY_LENGTH: one, where no sequence's
+// items are longer than four units (a block that takes several short items has
+// them one after the other).
+template <bool BY_LENGTH, typename Work>
 __device__ __forceinline__ AttnShare attn_share(const Work& w, int least, long long* sh) {
   const int threads = blockDim.x, batch = w.p.b.batch;
   const int per = (batch + threads - 1) / threads;
   const int b0 = min((int)threadIdx.x * per, batch), b1 = min(b0 + per, batch);
   long long sum = 0;
-  for (int b = b0; b < b1; ++b) sum += w.units(b);
+  bool longer = false;
+  for (int b = b0; b < b1; ++b) sum += w.units(b, BY_LENGTH ? &longer : nullptr);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long incl = sum;
 #pragma unroll
@@ -242,7 +247,10 @@ __device__ __forceinline__ AttnShare attn_share(const Work& w, int least, long l
     if (lane >= off) incl += o;
   }
   if (lane == 31) sh[warp] = incl;
-  __syncthreads();
+  if (!BY_LENGTH)
+    __syncthreads();
+  else if (!__syncthreads_or(longer))
+    least = 1;
   long long before = 0, total = 0;
   for (int i = 0; i < threads / 32; ++i) {
     if (i < warp) before += sh[i];
