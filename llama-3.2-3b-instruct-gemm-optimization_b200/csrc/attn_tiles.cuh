@@ -99,7 +99,7 @@ struct TilesKernel {
     uint32_t tmem;
     int last[2];
   };
-  static_assert(sizeof(Shared) <= 3072, "static shared memory");
+  static_assert(sizeof(Shared) <= 3 * 1024, "static shared memory");
 
   // Byte of 16-byte chunk c (of D / 8) of row r in a 16-bit tile.
   static __device__ __forceinline__ uint32_t chunk_at(int r, int c) {

@@ -82,6 +82,28 @@ def test_residual(b2g, cuda, m, n, k):
     check_product(b2g, m, n, k, "fp16", b2g.FUSE_RESIDUAL_ADD)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("m", [3, 300])
+def test_gates_far_from_zero(b2g, cuda, dtype, m):
+    """Gates to +-200, past where exp overflows.  The gate is off by 3 half
+    steps of fp32, its exponential by |g| times that, |g| 2^-24 for the argument
+    and 2 ulp, the division by 2 ulp: (|g| + 8) 2^-22 of the value; where
+    1 + exp(-g) passes 2^126 it may be 0, which is off by |g u| 2^-126."""
+    n, k, t = 300, 128, TYPES[dtype]
+    xq, wq = codes(m, k, 11), codes(2 * n, k, 12)
+    sx = torch.full((m,), 1 / 73.0, device="cuda")
+    sw = torch.cat([torch.full((n,), 60 / 73 / math.sqrt(k), device="cuda"),
+                    torch.full((n,), 1 / 73 / math.sqrt(k), device="cuda")])
+    op = b2g.I8Op(k, n, max_m=m, fuse=b2g.FUSE_GATE_UP_SILU, dtype=dtype)
+    y = op.enqueue_codes(xq, sx, wq, sw, workspace=op.workspace())
+    both = (xq.double() @ wq.double().T) * sx.double()[:, None] * sw.double()[None]
+    g, u = both[:, :n], both[:, n:]
+    assert float(g.min()) < -130 and float(g.max()) > 130
+    want = g * torch.sigmoid(g) * u
+    bound = (torch.finfo(t).eps / 2 + (g.abs() + 8) * 2.0 ** -22) * want.abs() + (g * u).abs() * 2.0 ** -126 + 2.0 ** -25
+    assert bool(((y.double() - want).abs() <= bound).all())
+
+
 def test_extreme_codes(b2g, cuda):
     """The largest sums: every product 127 * 127 or (-128) * (-128) at the
     largest k; one more k could reach 2^31 and is refused."""
