@@ -248,9 +248,7 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
             const float2 f = Act<T>::unpack(o[x]);
             o[x] = Act<__half>::pack(f.x * by, f.y * by);
           }
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + chunk_at(tid, ch)), "r"(o[0]), "r"(o[1]),
-                       "r"(o[2]), "r"(o[3])
-                       : "memory");
+          sts128_at(dst + chunk_at(tid, ch), make_uint4(o[0], o[1], o[2], o[3]));
         }
       }
     }
@@ -367,12 +365,8 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
             uint32_t o[8];
 #pragma unroll
             for (int x = 0; x < 4; ++x) e4m3x4_to_f16x2x2(wd[x], o[2 * x], o[2 * x + 1]);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + chunk_at(t, 2 * c)), "r"(o[0]), "r"(o[1]),
-                         "r"(o[2]), "r"(o[3])
-                         : "memory");
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + chunk_at(t, 2 * c + 1)), "r"(o[4]),
-                         "r"(o[5]), "r"(o[6]), "r"(o[7])
-                         : "memory");
+            sts128_at(dst + chunk_at(t, 2 * c), make_uint4(o[0], o[1], o[2], o[3]));
+            sts128_at(dst + chunk_at(t, 2 * c + 1), make_uint4(o[4], o[5], o[6], o[7]));
           }
           copy_next(sl);  // the slot's bytes are in the ring
           announce(&s.kv_full[st]);

@@ -267,6 +267,11 @@ __device__ __forceinline__ uint4 lds128_at(uint32_t a) {
   return v;
 }
 
+// The store beside it.
+__device__ __forceinline__ void sts128_at(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 __device__ __forceinline__ uint2 lds64_at(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
