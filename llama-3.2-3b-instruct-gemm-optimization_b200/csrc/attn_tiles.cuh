@@ -95,7 +95,11 @@ struct TilesKernel {
     long long share[kThreads / 32];
     long long row_at[2][kTile];  // the unit's tokens' rows in the cache, -1: none
     uint32_t there[8][4];        // bit t: token t of unit (u mod 8) is there
-    uint8_t q_exp[kRows];        // kScaleQ: exponent of the row's power of two
+    // kScaleQ: exponent of the row's power of two, by the segment's parity.  The
+    // next segment's q may be loaded as soon as this one's last Q K^T is done, and
+    // the softmax warps may still be writing the one before.  Of that one they have
+    // read theirs: its products waited for their P.
+    uint8_t q_exp[2][kRows];
     uint32_t tmem;
     int last[2];
   };
@@ -237,7 +241,7 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
         }
         const int e = (int)(top >> 7);  // bf16 exponent of the largest
         const int ue = e > 0 && e < 255 ? min(max(127 + 13 - (e - 127), 1), 253) : 127;
-        s.q_exp[r] = (uint8_t)ue;
+        s.q_exp[~n_q & 1][r] = (uint8_t)ue;  // n_q counts this one already
         const float by = __uint_as_float((uint32_t)ue << 23);
         for (int ch = 0; ch < D / 8; ++ch) {
           uint4 v = make_uint4(0, 0, 0, 0);
@@ -501,7 +505,7 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
   };
   uint32_t s_par[2] = {0, 0};
   int n = 0;  // units of this block so far
-  while (k.next()) {
+  for (int seg = 0; k.next(); ++seg) {
     const int rows = k.rows();
     if (tile * kTile >= rows) {
       n += k.units;
@@ -528,7 +532,7 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
       tmem_ld32(at, x[0]);
       tmem_ld32(at + 32, x[1]);
       if constexpr (kScaleQ) {
-        if (u == 0) scale *= 1.0f / __uint_as_float((uint32_t)s.q_exp[r] << 23);
+        if (u == 0) scale *= 1.0f / __uint_as_float((uint32_t)s.q_exp[seg & 1][r] << 23);
       }
       const uint2 there = *reinterpret_cast<const uint2*>(&s.there[(n + (u >> 1)) & 7][2 * half]);
       const bool masked = (there.x & there.y) != 0xffffffffu || j0 + kStep - 1 > first_pos || j0 <= last_low;

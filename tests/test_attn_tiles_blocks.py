@@ -154,3 +154,10 @@ def run(program, types, batch, sleepiness, seeds):
 @pytest.mark.parametrize("types", TYPES[1:])
 def test_warps_in_even_turns(program, types, batch):
     run(program, types, batch, 0, 2)
+
+
+def test_scales_of_rows_outlive_the_next_loads(program):
+    """bf16 rows over an 8-bit cache, each in a range of its own: a block that
+    takes several items of one unit keeps an item's scales until its softmax has
+    read them, however far the loads and products are ahead."""
+    run(program, TYPES[0], BATCHES[0], 0, 5)
