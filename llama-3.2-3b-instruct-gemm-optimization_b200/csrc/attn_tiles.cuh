@@ -22,7 +22,10 @@
 // softmax gets to them, so neither side waits for the other's latency (with
 // one buffer of 128 columns a unit took 4650 clocks, 1800 of them from a P to
 // the next S).  A tile's S(u + 2) is issued behind its O += P(u) V(u) into the
-// same buffer and one commit covers both.
+// same buffer and one commit covers both.  An item's last two O += P V have a
+// barrier of their own: the next item's S is issued without a word from the
+// softmax warps, and on s_full its phase could end before a warp that stood
+// still had seen theirs.
 // Three chunks of up to 2048 tokens at up to 6000, 32 heads on 8, bf16: 388 us in
 // a short run, 0.91 PFLOP/s (436 in a long one at the power limit);
 // the softmax warps take 2000 clocks for 64 columns of both tiles, of which
@@ -91,7 +94,8 @@ struct TilesKernel {
   using P16 = typename std::conditional<kBf16, __nv_bfloat16, __half>::type;
 
   struct Shared {
-    uint64_t kv_full[kStages], kv_empty[kStages], q_full, q_empty, s_full[2][2], p_full[2][2], drain[2];
+    uint64_t kv_full[kStages], kv_empty[kStages], q_full, q_empty, s_full[2][2], p_full[2][2], o_full[2][2],
+        drain[2];
     long long share[kThreads / 32];
     long long row_at[2][kTile];  // the unit's tokens' rows in the cache, -1: none
     uint32_t there[8][4];        // bit t: token t of unit (u mod 8) is there
@@ -469,7 +473,7 @@ __device__ void TilesKernel<T, FP8, D>::multiply(const AttnParams& p, Shared& s,
           wait(&s.p_full[t][half], p_par);
           pv(vp, half, j == 0 && half == 0);
           if (!last) qk(kp, half);
-          tc_commit(&s.s_full[t][half]);  // the next scores, or (the last time) O
+          tc_commit(last ? &s.o_full[t][half] : &s.s_full[t][half]);
         }
         p_par ^= 1;
       }
@@ -503,7 +507,7 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
     __syncwarp();
     tc_fence_after();
   };
-  uint32_t s_par[2] = {0, 0};
+  uint32_t s_par[2] = {0, 0}, o_par = 0;
   int n = 0;  // units of this block so far
   for (int seg = 0; k.next(); ++seg) {
     const int rows = k.rows();
@@ -562,8 +566,10 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
           const float by = grown ? exp2_fast(m - top) : 1.0f;
           if (grown) m = top;
           l *= by;
-          // The other buffer's next phase comes behind the last step's products.
-          wait(&s.s_full[tile][half ^ 1], s_par[half ^ 1]);
+          // Behind the last step's products comes the other buffer's next phase,
+          // or the first of the item's last two.
+          if (u + 1 < 2 * k.units) wait(&s.s_full[tile][half ^ 1], s_par[half ^ 1]);
+          else wait(&s.o_full[tile][0], o_par);
 #pragma unroll 1
           for (int i = 0; i < D / 16; ++i) {
             uint32_t o[16];
@@ -596,11 +602,8 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
       mbar_arrive(&s.p_full[tile][half]);
     }
     n += k.units;
-    // Each buffer's last phase: O is complete.
-    wait(&s.s_full[tile][0], s_par[0]);
-    wait(&s.s_full[tile][1], s_par[1]);
-    s_par[0] ^= 1;
-    s_par[1] ^= 1;
+    wait(&s.o_full[tile][1], o_par);  // all of the item's products
+    o_par ^= 1;
 
     const float vs = FP8 && p.c.v_scale ? p.c.v_scale[k.it.h] : 1.0f;
     const long long t = k.it.s.first + tok;
@@ -717,6 +720,7 @@ __global__ void __launch_bounds__(512, 1) attn_tiles_kernel(const __grid_constan
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s.s_full[i >> 1][i & 1], 1);
       mbar_init(&s.p_full[i >> 1][i & 1], 128);
+      mbar_init(&s.o_full[i >> 1][i & 1], 1);
     }
     mbar_init(&s.drain[0], 1);
     mbar_init(&s.drain[1], 1);

@@ -161,3 +161,11 @@ def test_scales_of_rows_outlive_the_next_loads(program):
     takes several items of one unit keeps an item's scales until its softmax has
     read them, however far the loads and products are ahead."""
     run(program, TYPES[0], BATCHES[0], 0, 5)
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("types", TYPES)
+def test_warps_that_stand_still(program, types, batch):
+    """One arrival in 3000 sends its warp to sleep for up to 4000 turns: no phase
+    of a barrier may pass before all who wait for it have seen it."""
+    run(program, types, batch, 3000, 10)
