@@ -507,7 +507,7 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
     __syncwarp();
     tc_fence_after();
   };
-  uint32_t s_par[2] = {0, 0}, o_par = 0;
+  uint32_t par = 0;  // of s_full[0], s_full[1] and o_full, a bit each (a register each: 341 us against 327, D = 64)
   int n = 0;  // units of this block so far
   for (int seg = 0; k.next(); ++seg) {
     const int rows = k.rows();
@@ -530,8 +530,8 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
       const int half = u & 1;
       const int j0 = k.u0 * kUnit + u * kStep;
       const uint32_t at = tm_s + half * kStep;
-      wait(&s.s_full[tile][half], s_par[half]);
-      s_par[half] ^= 1;
+      wait(&s.s_full[tile][half], par >> half & 1);
+      par ^= 1 << half;
       uint32_t x[2][32];
       tmem_ld32(at, x[0]);
       tmem_ld32(at + 32, x[1]);
@@ -568,8 +568,8 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
           l *= by;
           // Behind the last step's products comes the other buffer's next phase,
           // or the first of the item's last two.
-          if (u + 1 < 2 * k.units) wait(&s.s_full[tile][half ^ 1], s_par[half ^ 1]);
-          else wait(&s.o_full[tile][0], o_par);
+          if (u + 1 < 2 * k.units) wait(&s.s_full[tile][half ^ 1], par >> (half ^ 1) & 1);
+          else wait(&s.o_full[tile][0], par >> 2);
 #pragma unroll 1
           for (int i = 0; i < D / 16; ++i) {
             uint32_t o[16];
@@ -602,8 +602,8 @@ __device__ void TilesKernel<T, FP8, D>::softmax(const AttnParams& p, Shared& s, 
       mbar_arrive(&s.p_full[tile][half]);
     }
     n += k.units;
-    wait(&s.o_full[tile][1], o_par);  // all of the item's products
-    o_par ^= 1;
+    wait(&s.o_full[tile][1], par >> 2);  // all of the item's products
+    par ^= 4;
 
     const float vs = FP8 && p.c.v_scale ? p.c.v_scale[k.it.h] : 1.0f;
     const long long t = k.it.s.first + tok;
