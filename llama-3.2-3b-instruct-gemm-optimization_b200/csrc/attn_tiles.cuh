@@ -30,8 +30,11 @@
 // a short run, 0.91 PFLOP/s (436 in a long one at the power limit);
 // the softmax warps take 2000 clocks for 64 columns of both tiles, of which
 // the exponentials are 1024.
-// Every wait is bounded; after one has run out its thread goes through the
-// remaining steps without waiting, so that barriers still meet.
+// Every wait is bounded.  After one has run out a products' warp is done; a thread
+// of the others goes through the remaining steps without waiting, so that their
+// barriers still meet (the loads without issuing or announcing anything, which a
+// barrier's later phase would count).  The block ends behind the copies and
+// products that it has issued.
 #pragma once
 #include "attn_rows.cuh"
 #include "tc.cuh"
@@ -225,6 +228,7 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
       wait(&s.q_empty, (n_q - 1) & 1);
     }
     ++n_q;
+    if (!ok) return;
     const int rows = k.rows();
     for (int i = 0; i < 2; ++i) {
       const int r = i * 128 + tid, abs_r = k.it.tile * kRows + r;
@@ -287,6 +291,7 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
       look_up_box(n, unit);
       note(n, look_up(k.it, unit));
     };
+    int sent = 0;  // tiles before a wait ran out
     if (more) prepare(0, k.u0);
     for (int n = 1; more; ++n) {  // the unit whose rows are looked up next
       const int units = k.units;
@@ -303,23 +308,26 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
               wait(&s.kv_empty[st], parity);
             }
           }
+          if (ok) sent = tiles + 1;
           ++tiles;
           uint64_t* full = &s.kv_full[st];
           const uint32_t dst = smem + kOffRing + st * kTileBytes;
           if (whole) {
-            if (tid == 0) mbar_arrive_expect_tx(full, kTileBytes);
-            else mbar_arrive(full);
+            if (ok) {
+              if (tid == 0) mbar_arrive_expect_tx(full, kTileBytes);
+              else mbar_arrive(full);
+            }
             __syncwarp();
-            if (warp == 0 && box < boxes)
+            if (warp == 0 && box < boxes && ok)
               tma_load_4d(dst + panel * kPanelBytes + box * tma.box_rows * 128, kv == 0 ? &tma.k : &tma.v, panel * 64,
                           (n & 1) ? box_row[0] : box_row[1], k.it.h, (n & 1) ? box_page[0] : box_page[1], full);
-          } else {
+          } else if (ok) {
             copy_tile(n - 1, kv == 0 ? p.c.k : p.c.v, dst, false);
             commit(full);
           }
           if (j == 0 && kv == 0) {
             load_q(k);
-            commit(&s.q_full);
+            if (ok) commit(&s.q_full);
           }
         }
         if (whole) flush();  // copies behind which none may come for long
@@ -330,6 +338,12 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
       if (more) prepare(n, k.u0);
     }
     flush();
+    // Whoever was to use them may have given up: bulk copies land before this
+    // block's memory goes.
+    bool landed = true;
+    for (int j = max(0, sent - kStages); j < sent; ++j)
+      landed = landed && mbar_wait_spin(&s.kv_full[j % kStages], (j / kStages) & 1);
+    if (!landed) *p.error = kErrDrainWait;
   } else {
     // 8-bit: copies run two tiles ahead into private staging slots (a thread
     // widens what it has copied itself).
@@ -377,12 +391,12 @@ __device__ void TilesKernel<T, FP8, D>::load(const AttnTma& tma, const AttnParam
             sts128_at(dst + chunk_at(t, 2 * c + 1), make_uint4(o[4], o[5], o[6], o[7]));
           }
           copy_next(sl);  // the slot's bytes are in the ring
-          announce(&s.kv_full[st]);
+          if (ok) announce(&s.kv_full[st]);
           if (j == 0 && kv == 0) {
             load_q(k);
             cp_async_commit();
             cp_async_wait<0>();
-            announce(&s.q_full);
+            if (ok) announce(&s.q_full);
           }
         }
     }
@@ -400,13 +414,11 @@ __device__ void TilesKernel<T, FP8, D>::multiply(const AttnParams& p, Shared& s,
   constexpr uint32_t kQk = tc_idesc(1, kFmt, kFmt, 0, kStep), kPv = tc_idesc(1, kFmt, kFmt, 1, D);
   const Work w(p);
   AttnWalk<Work> k(w, share);
-  bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok && !mbar_wait_spin(bar, parity)) {
-      *p.error = kErrFullWait;
-      ok = false;
-    }
+    const bool ok = mbar_wait_spin(bar, parity);
+    if (!ok) *p.error = kErrFullWait;
     tc_fence_after();
+    return ok;
   };
   const uint32_t tm = s.tmem;
   // Places in the ring, kept by counting: this thread's own instructions are
@@ -424,7 +436,6 @@ __device__ void TilesKernel<T, FP8, D>::multiply(const AttnParams& p, Shared& s,
   const uint64_t q_desc = smem_desc_sw128(smem, 16, 1024), k_desc = smem_desc_sw128(smem + kOffRing, 16, 1024),
                  v_desc = smem_desc_sw128(smem + kOffRing, kPanelBytes, 1024);
   auto qk = [&](const Place& at, int half) {  // S_t[half] = Q_t (half of K)^T
-    if (!ok) return;
     const uint64_t a = q_desc + t * (kTileBytes >> 4), b = k_desc + at.st * (kTileBytes >> 4) + half * (kStep * 128 >> 4);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
@@ -433,59 +444,61 @@ __device__ void TilesKernel<T, FP8, D>::multiply(const AttnParams& p, Shared& s,
     }
   };
   auto pv = [&](const Place& at, int half, bool first) {  // O_t (+)= P_t[half] (half of V)
-    if (!ok) return;
     const uint64_t b = v_desc + at.st * (kTileBytes >> 4) + half * (kStep * 128 >> 4);
 #pragma unroll
     for (int ks = 0; ks < kStep / 16; ++ks)
       mma_f16_ts(tm + 2 * kUnit + t * D, tm + t * kUnit + half * kStep + ks * 8, b + ((ks * 2048) >> 4), kPv,
                  !first || ks > 0);
   };
-  Place kp;  // of the next keys
-  uint32_t q_par = 0, p_par = 0;
-  while (k.next()) {
-    const bool mine = t * kTile < k.rows();  // else this warp only hands the stages back
-    const int units = k.units;
-    auto give_back = [&](uint64_t* bar) {
-      if (mine) tc_commit(bar);
-      else mbar_arrive(bar);
-    };
-    wait(&s.q_full, q_par);
-    q_par ^= 1;
-    wait(&s.kv_full[kp.st], kp.parity);
-    if (mine) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        qk(kp, half);
-        tc_commit(&s.s_full[t][half]);
-      }
-    }
-    give_back(&s.kv_empty[kp.st]);
-    if (units == 1) give_back(&s.q_empty);
-    for (int j = 0; j < units; ++j) {
-      const bool last = j + 1 == units;
-      const Place vp = kp.after();
-      kp = vp.after();
-      wait(&s.kv_full[vp.st], vp.parity);
-      if (!last) wait(&s.kv_full[kp.st], kp.parity);
+  auto run = [&]() {  // false: a wait ran out
+    Place kp;  // of the next keys
+    uint32_t q_par = 0, p_par = 0;
+    while (k.next()) {
+      const bool mine = t * kTile < k.rows();  // else this warp only hands the stages back
+      const int units = k.units;
+      auto give_back = [&](uint64_t* bar) {
+        if (mine) tc_commit(bar);
+        else mbar_arrive(bar);
+      };
+      if (!wait(&s.q_full, q_par)) return false;
+      q_par ^= 1;
+      if (!wait(&s.kv_full[kp.st], kp.parity)) return false;
       if (mine) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          wait(&s.p_full[t][half], p_par);
-          pv(vp, half, j == 0 && half == 0);
-          if (!last) qk(kp, half);
-          tc_commit(last ? &s.o_full[t][half] : &s.s_full[t][half]);
+          qk(kp, half);
+          tc_commit(&s.s_full[t][half]);
         }
-        p_par ^= 1;
       }
-      give_back(&s.kv_empty[vp.st]);
-      if (!last) give_back(&s.kv_empty[kp.st]);
-      if (j + 2 == units) give_back(&s.q_empty);
+      give_back(&s.kv_empty[kp.st]);
+      if (units == 1) give_back(&s.q_empty);
+      for (int j = 0; j < units; ++j) {
+        const bool last = j + 1 == units;
+        const Place vp = kp.after();
+        kp = vp.after();
+        if (!wait(&s.kv_full[vp.st], vp.parity)) return false;
+        if (!last && !wait(&s.kv_full[kp.st], kp.parity)) return false;
+        if (mine) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!wait(&s.p_full[t][half], p_par)) return false;
+            pv(vp, half, j == 0 && half == 0);
+            if (!last) qk(kp, half);
+            tc_commit(last ? &s.o_full[t][half] : &s.s_full[t][half]);
+          }
+          p_par ^= 1;
+        }
+        give_back(&s.kv_empty[vp.st]);
+        if (!last) give_back(&s.kv_empty[kp.st]);
+        if (j + 2 == units) give_back(&s.q_empty);
+      }
     }
-  }
-  if (!ok) {
-    tc_commit(&s.drain[t]);
-    mbar_wait_spin(&s.drain[t], 0);
-  }
+    return true;
+  };
+  run();
+  // The softmax warps may have given up: products end before tensor memory goes.
+  tc_commit(&s.drain[t]);
+  if (!mbar_wait_spin(&s.drain[t], 0)) *p.error = kErrDrainWait;
 }
 
 // ---------------------------------------------------------------------------

@@ -8,8 +8,8 @@
 // place, and how long a warp stands still is drawn from a seed, so that orders
 // that a GPU takes once in a million launches come up.  What is checked on the
 // way: a phase of an mbarrier gets no more arrivals than it has room for, the
-// lanes of a warp meet in the same collective, and nothing that was issued is
-// still on its way when the block has ended.
+// lanes of a warp meet in the same collective, and no copy or product is still on
+// its way when the block has ended.  Waits can be made to run out, too.
 #pragma once
 #include <cstddef>
 #include <cstdint>
@@ -86,7 +86,7 @@ struct Thread {
   struct Copy { uint32_t dst; const void* src; bool in; };
   std::vector<std::vector<Copy>> groups;  // of 16-byte copies, committed
   std::vector<Copy> open;
-  struct Op { std::function<void()> run; };
+  struct Op { std::function<void()> run; bool commit; };
   std::deque<Op> tensor;  // matrix products and commits, in order
 };
 inline std::vector<Thread> threads;
@@ -97,7 +97,7 @@ inline std::vector<std::function<void()>> bulk;  // bulk copies on their way
 struct NamedBar { int count = 0; bool any = false; };
 inline NamedBar named[16];
 inline int sleepiness = 0;  // one in how many arrivals sends its warp to sleep (0: none)
-inline std::function<bool(void*, int)> expire;  // whether this wait of this thread runs out
+inline std::function<bool(int)> expire;  // whether this wait of a thread runs out though its phase ends
 
 inline Thread& self() { return threads[current]; }
 inline void yield() { swapcontext(&self().ctx, &main_ctx); }
@@ -219,7 +219,7 @@ inline void run_block(int n_threads, const std::function<void()>& body) {
       }
       ready.push_back(i);
     }
-    if (!live && !units) break;
+    if (!live) break;
     if (units && (ready.empty() || draw(4) == 0)) {
       const unsigned pick = draw(units);
       if (pick < issuers.size()) {
@@ -234,10 +234,6 @@ inline void run_block(int n_threads, const std::function<void()>& body) {
         op();
       }
       continue;
-    }
-    if (!live) {
-      fail("copies or products on their way when the block ended");
-      break;
     }
     if (ready.empty()) {
       if (asleep) {  // all others wait for the sleepers
@@ -259,8 +255,10 @@ inline void run_block(int n_threads, const std::function<void()>& body) {
       swapcontext(&main_ctx, &threads[i].ctx);
     }
   }
+  if (!bulk.empty()) fail("bulk copies on their way when the block ended");
   for (Thread& t : threads) {
-    if (!t.tensor.empty()) fail("products on their way when the block ended");
+    for (auto& op : t.tensor)
+      if (!op.commit) fail("products on their way when the block ended");
     for (auto& g : t.groups)
       if (!g.empty()) fail("copies on their way when the block ended");
   }
@@ -338,7 +336,7 @@ inline void mbar_arrive_expect_tx(uint64_t* b, uint32_t bytes) {
 inline bool mbar_test(uint64_t* b, uint32_t parity) { return emu::passed(bar_of(b), parity); }
 inline bool mbar_wait_spin(uint64_t* b, uint32_t parity) {
   emu::Thread& t = emu::self();
-  if (emu::expire && emu::expire(b, emu::current)) return false;
+  if (emu::expire && emu::expire(emu::current)) return false;
   t.bar = bar_of(b);
   t.parity = parity & 1;
   t.expired = false;
@@ -421,7 +419,9 @@ inline float f16_value(uint16_t v, bool bf16) {
   h.x = v;
   return __half2float(__half(h));
 }
-inline void issue(std::function<void()> f) { emu::self().tensor.push_back({std::move(f)}); }
+inline void issue(std::function<void()> f, bool commit = false) {
+  emu::self().tensor.push_back({std::move(f), commit});
+}
 inline void f16_product(uint32_t d, const float* a, uint64_t b, uint32_t idesc, bool accumulate) {
   const int n = (idesc >> 17 & 63) * 8;
   const bool bf16 = idesc >> 10 & 7, mn = idesc >> 16 & 1;
@@ -478,7 +478,7 @@ inline void mma_i8_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool a
   });
 }
 inline void tc_commit(uint64_t* b) {
-  issue([=] { emu::arrive(bar_of(b)); });
+  issue([=] { emu::arrive(bar_of(b)); }, true);
 }
 inline void fence_proxy_async_shared() {}
 

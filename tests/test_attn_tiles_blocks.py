@@ -21,6 +21,9 @@ static double value(__half v) { return __half2float(v); }
 static double value(__nv_bfloat16 v) { return __bfloat162float(v); }
 static double value(uint8_t v) { return __half2float(__half(__half_raw(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)))); }
 
+// first .. last: threads whose `late`th wait runs out (none: first < 0).
+static int first = -1, last = -1, late = 0;
+
 template <typename T, bool FP8, int D>
 int run(std::vector<int> fresh, std::vector<int> total, int kv_heads, int group, int page, int grid, int least) {
   using K = TilesKernel<T, FP8, D>;
@@ -71,9 +74,13 @@ int run(std::vector<int> fresh, std::vector<int> total, int kv_heads, int group,
   emu::gridDim_.x = grid;
   for (int c = 0; c < grid; ++c) {
     emu::blockIdx_.x = c;
+    std::vector<int> waits(K::kThreads);
+    emu::expire = nullptr;
+    if (first >= 0) emu::expire = [&](int i) { return i >= first && i <= last && ++waits[i] == late; };
     emu::run_block(K::kThreads, [&] { attn_tiles_kernel<T, FP8, D>(a); });
     if (emu::failure) return printf("block %d: %s\n", c, emu::failure), 1;
   }
+  if (first >= 0) return error ? 0 : (printf("no error is set\n"), 1);
   if (error) return printf("error word %d\n", error), 1;
   for (int c : counters)
     if (c) return printf("counters are left dirty\n"), 1;
@@ -114,6 +121,7 @@ int main(int argc, char** argv) {
   for (int seed = 1; seed <= atoi(argv[4]); ++seed) {
     emu::rng_state = seed;
     emu::sleepiness = sleepy;
+    if (argc > 5) first = atoi(argv[5]), last = atoi(argv[6]), late = 1 + (seed - 1) % atoi(argv[7]);
     std::vector<int> fresh, total;
     int least = 1, grid = 2;
     if (batch == 0) {  // short prompts: several items of one unit a block
@@ -144,8 +152,8 @@ TYPES = ["bf16 over e4m3", "bf16", "fp16 over e4m3", "fp16"]
 BATCHES = ["short prompts", "a long one ahead"]
 
 
-def run(program, types, batch, sleepiness, seeds):
-    args = [TYPES.index(types), BATCHES.index(batch), sleepiness, seeds]
+def run(program, types, batch, sleepiness, seeds, *expire):
+    args = [TYPES.index(types), BATCHES.index(batch), sleepiness, seeds, *expire]
     out = subprocess.run([str(program), *map(str, args)], capture_output=True, text=True)
     assert out.returncode == 0 and out.stdout == "ok\n", out.stdout + out.stderr
 
@@ -169,3 +177,13 @@ def test_warps_that_stand_still(program, types, batch):
     """One arrival in 3000 sends its warp to sleep for up to 4000 turns: no phase
     of a barrier may pass before all who wait for it have seen it."""
     run(program, types, batch, 3000, 10)
+
+
+@pytest.mark.parametrize("threads", [(0, 31), (5, 5), (128, 255), (256, 383), (256, 256), (300, 300), (384, 384), (416, 416)],
+                         ids=["a softmax warp", "a softmax lane", "a tile's softmax", "the loads", "the first load lane",
+                              "another load lane", "products of tile 0", "products of tile 1"])
+@pytest.mark.parametrize("types", TYPES)
+def test_waits_that_run_out(program, types, threads):
+    """Whichever wait of these threads runs out: the block ends, with an error
+    set, and no copy or product is on its way behind it."""
+    run(program, types, BATCHES[1], 0, 6, *threads, 6)
