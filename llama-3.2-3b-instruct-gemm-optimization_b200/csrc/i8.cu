@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kI8MaxStages], empty[kI8MaxStages], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_base_sh;
-  __shared__ int last_sh;
+  __shared__ int last_sh, gave_up_sh;
   __shared__ __align__(16) float sx_sh[2][256];
   uint8_t* ring = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -334,7 +334,13 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
     }
     mbar_init(&drain, 1);
     fence_mbarrier_init();
+    gave_up_sh = 0;
   }
+  int sent = 0;  // thread 0: k blocks asked for
+  auto give_up = [&](int code) {
+    *t.error = code;
+    gave_up_sh = 1;
+  };
   if (warp == 1) tmem_alloc(&tmem_base_sh, t.tmem_cols);
   tc_fence_before();
   __syncthreads();
@@ -376,7 +382,7 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
           const int stage = i % t.stages;
           if (i >= issued) {
             if (i >= t.stages && !mbar_wait_spin(&empty[stage], (i / t.stages - 1) & 1)) {
-              *t.error = kErrEmptyWait;
+              give_up(kErrEmptyWait);
               ok = false;
               break;
             }
@@ -385,9 +391,7 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
           }
           load_x(stage, s, k);
         }
-      // After an error the copies in flight land before this CTA's memory goes.
-      if (!ok)
-        for (int j = max(0, i - t.stages); j < i; ++j) mbar_wait_spin(&full[j % t.stages], (j / t.stages) & 1);
+      sent = i;
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
       while (ok && s.next(t)) {
         const int buf = n % kBufs;
         if (!mbar_wait_spin(&acc_empty[buf], ((n / kBufs) & 1) ^ 1)) {
-          *t.error = kErrEmptyWait;
+          give_up(kErrEmptyWait);
           ok = false;
           break;
         }
@@ -408,7 +412,7 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
         for (int k = s.k0; k < s.k1; ++k, ++i) {
           const int stage = i % t.stages;
           if (!mbar_wait_spin(&full[stage], (i / t.stages) & 1)) {
-            *t.error = kErrFullWait;
+            give_up(kErrFullWait);
             ok = false;
             break;
           }
@@ -428,10 +432,6 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
         if (ok) tc_commit(&acc_full[buf]);
         ++n;
       }
-      if (!ok) {
-        tc_commit(&drain);
-        mbar_wait_spin(&drain, 0);
-      }
     }
   } else {
     pdl_wait();
@@ -443,6 +443,9 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
     I8Seg s;
     s.begin(t);
     int n = 0;
+    // After a wait that has run out its thread goes through the remaining pieces
+    // without waiting, so that barriers and warp-wide instructions still meet.
+    bool ok = true;
     while (s.next(t)) {
       const int buf = n % kBufs;
       const int tok0 = s.tile % t.tok_tiles * t.bn, j = s.tile / t.tok_tiles * kChannels + ch;
@@ -479,10 +482,11 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
       };
       if (t.cluster == 1) load_residual(first);
       named_sync(1, kEpi);
-      if (!mbar_wait_spin(&acc_full[buf], (n / kBufs) & 1)) {
-        *t.error = kErrFullWait;
-        break;
+      if (ok && !mbar_wait_spin(&acc_full[buf], (n / kBufs) & 1)) {
+        give_up(kErrFullWait);
+        ok = false;
       }
+      __syncwarp();
       tc_fence_after();
       // Columns go 32 at a time; those behind the last row are read (scratch or
       // a clamped row) and not stored, so that no load waits on a branch.
@@ -639,6 +643,20 @@ __global__ void __launch_bounds__(DEEP ? 320 : 192, 1) i8_product_kernel(const _
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (gave_up_sh) {
+    // Nobody may have waited for what is on its way: copies and products end
+    // before shared and tensor memory go.
+    bool ok = true;
+    if (threadIdx.x == 0)
+      for (int i = max(0, sent - t.stages); i < sent; ++i)
+        ok = ok && mbar_wait_spin(&full[i % t.stages], (i / t.stages) & 1);
+    if (threadIdx.x == 32) {
+      tc_commit(&drain);
+      ok = mbar_wait_spin(&drain, 0);
+    }
+    if (!ok) *t.error = kErrDrainWait;
+    __syncwarp();
+  }
   if (warp == 1) tmem_dealloc(tmem, t.tmem_cols);
 }
 

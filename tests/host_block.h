@@ -287,6 +287,7 @@ inline uint32_t __float_as_uint(float f) { uint32_t u; memcpy(&u, &f, 4); return
 inline float __uint_as_float(uint32_t u) { float f; memcpy(&f, &u, 4); return f; }
 inline uint32_t __byte_perm(uint32_t, uint32_t, uint32_t) { abort(); }
 inline int __popc(uint32_t v) { return __builtin_popcount(v); }
+inline float rsqrtf(float v) { return 1 / sqrtf(v); }
 inline float __expf(float v) { return expf(v); }
 inline float __fdividef(float a, float b) { return b > 0x1p126f && b < INFINITY ? a * 0.f : a / b; }
 template <typename T> inline T __ldcg(const T* p) { return *p; }
