@@ -160,6 +160,35 @@ def test_bad_pages_are_not_written(b2g, cuda):
     assert b2g.device_error() == 6  # past the table
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_8bit_codes_are_the_rounded_quotients(b2g, cuda, dtype):
+    """Codes of value / scale, divided in fp32 and rounded once: ties
+    (which a product by 1 / scale leaves on either side), neighbours of ties,
+    saturation, and scales whose reciprocal fp32 does not hold."""
+    t, d = TYPES[dtype], 64
+    scales = [m / 64 for m in range(33, 64, 2)] + [m / 7 for m in range(1, 9)] + [1e-39, 2e-38, 1e-30, 1e30, 3e38, 1.0]
+    ties = [m * 2.0 ** e for m in range(17, 32, 2) for e in range(-11, 5)] + [m * 2.0 ** -10 for m in range(1, 16, 2)]
+    s = torch.tensor(scales, dtype=torch.float32)
+    v = (torch.tensor(ties, dtype=torch.float64)[:, None] * s.double()).float().to(t)  # exact on a tie or next to it
+    g = torch.Generator().manual_seed(4)
+    v = torch.cat([v, -v, torch.randn(300, len(scales), generator=g).to(t), torch.zeros(4, len(scales)).to(t)])
+    v = v.nan_to_num(posinf=1.0, neginf=-1.0)
+    rows = -(-v.shape[0] // d)
+    x = torch.zeros(rows * d, len(scales), dtype=t)
+    x[:v.shape[0]] = v
+    x = x.view(rows, d, len(scales)).transpose(1, 2).contiguous()  # [rows, heads, dim], a scale a head
+    want = (x.float() / s[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn).float()
+    kc, vc = (torch.zeros(-(-rows // 16), 16, len(scales), d, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)
+              for _ in range(2))
+    cache = b2g.PagedCache(kc, vc, k_scale=s.cuda(), v_scale=s.cuda())
+    args = (torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([0, rows], [rows], [list(range(kc.shape[0]))]))
+    b2g.kv_append(x.cuda(), x.cuda(), cache, *args)
+    torch.cuda.synchronize()
+    for c in (kc, vc):
+        got = c.float().flatten(0, 1)[:rows].cpu()
+        assert torch.equal(got, want), f"{int((got != want).sum())} of {want.numel()} codes differ"
+
+
 def test_refusals(b2g, cuda):
     kc, vc = (torch.zeros(4, 16, 2, 64, device="cuda", dtype=torch.float16) for _ in range(2))
     cache = b2g.PagedCache(kc, vc)
