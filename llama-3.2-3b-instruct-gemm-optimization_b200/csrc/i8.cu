@@ -304,9 +304,12 @@ template <bool GATE>
 __device__ __forceinline__ float i8_value(int acc, int acc_up, float sw, float sw_up, float sx) {
   const float v = (float)acc * sw * sx;
   if constexpr (!GATE) return v;
-  // Within 2 ulp in fp32; 0 where 1 + exp(-v) passes 2^126.  (The division
+  // v / (1 + exp(-v)), for v < 0 as v exp(v) / (1 + exp(v)): the divisor is at most
+  // 2 (past 2^126 the fast division gives 0).  Off by (|v| + 8) 2^-22 of the value at
+  // most: the exponential's argument is rounded, the rest is a few ulp.  (The division
   // rounded to nearest made a gate||up product of 2048 x 8192 x 4096 1.4 times slower.)
-  return __fdividef(v, 1.0f + __expf(-v)) * ((float)acc_up * sw_up * sx);
+  const float e = __expf(-fabsf(v));
+  return __fdividef(v < 0.0f ? v * e : v, 1.0f + e) * ((float)acc_up * sw_up * sx);
 }
 
 // PLANES 128-row weight tiles a stage: gate and up (GATE), or two channel tiles.

@@ -104,6 +104,24 @@ def test_gates_far_from_zero(b2g, cuda, dtype, m):
     assert bool(((y.double() - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("m", [3, 300])
+def test_gates_whose_exponential_is_large(b2g, cuda, m):
+    """Gates of -60 to -100 under an up of 10^30: their SiLU is down to 10^-42, but
+    the product is a plain bf16 number.  The bound is test_gates_far_from_zero's;
+    below 2^-126 the exponential has steps of 2^-149."""
+    n, k = 300, 128
+    g = -60 - 40 * torch.arange(n, device="cuda").float() / n
+    sw = torch.cat([-g / k, torch.full((n,), 1e30 / k, device="cuda")])
+    xq, wq = torch.ones(m, k, dtype=torch.int8, device="cuda"), torch.ones(2 * n, k, dtype=torch.int8, device="cuda")
+    wq[:n] = -1
+    op = b2g.I8Op(k, n, max_m=m, fuse=b2g.FUSE_GATE_UP_SILU, dtype="bf16")
+    y = op.enqueue_codes(xq, torch.ones(m, device="cuda"), wq, sw)
+    gate, up = -k * sw[:n].double(), k * sw[n:].double()
+    want = gate * torch.sigmoid(gate) * up
+    bound = (2.0 ** -8 + (gate.abs() + 8) * 2.0 ** -22) * want.abs() + (gate * up).abs() * 2.0 ** -148
+    assert bool(((y.double() - want).abs() <= bound).all())
+
+
 def test_extreme_codes(b2g, cuda):
     """The largest sums: every product 127 * 127 or (-128) * (-128) at the
     largest k; one more k could reach 2^31 and is refused."""
