@@ -1,5 +1,6 @@
 // attention.cu -- attention of new tokens over a paged key/value cache: which
 // kernel a call takes, and its launch.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_rows.cuh"
@@ -75,13 +76,20 @@ cudaError_t launch_typed(const AttnParams& p, int num_sms, cudaStream_t stream) 
 
 }  // namespace
 
-size_t attn_counter_bytes(int num_sms) { return ((size_t)num_sms * 3 * 4 + 255) / 256 * 256; }
+// A counter a block of the rows kernel, and a tile and block (one an SM) of the
+// tiles kernel; two parts for each.
+size_t attn_counter_bytes(int num_sms) {
+  static_assert(RowsKernel<__half, false, 64>::kBlocks <= kAttnBlocks && RowsKernel<__half, true, 128>::kBlocks <= kAttnBlocks,
+                "a block's counters and parts");
+  return ((size_t)num_sms * std::max(kAttnBlocks, kAttnTiles) * 4 + 255) / 256 * 256;
+}
 size_t attn_part_bytes(int num_sms, int head_dim) {
-  const size_t rows = 3 * (size_t)(head_dim * 16 + 32), tiles = 2 * (size_t)(head_dim * 128 + 256);
+  const size_t rows = kAttnBlocks * (size_t)(head_dim * 16 + 32), tiles = kAttnTiles * (size_t)(head_dim * 128 + 256);
   static_assert(RowsKernel<__half, false, 64>::kPartFloats == 64 * 16 + 32 &&
-                    TilesKernel<__half, false, 64>::kPartFloats == 64 * 128 + 256,
+                    TilesKernel<__half, false, 64>::kPartFloats == 64 * 128 + 256 &&
+                    TilesKernel<__half, false, 64>::kRows == kAttnTiles * TilesKernel<__half, false, 64>::kTile,
                 "a block's parts");
-  return (size_t)num_sms * 2 * (rows > tiles ? rows : tiles) * 4;
+  return (size_t)num_sms * 2 * std::max(rows, tiles) * 4;
 }
 
 cudaError_t launch_attention(const AttnParams& p, int num_sms, cudaStream_t stream) {

@@ -71,7 +71,7 @@ struct RowsKernel {
   static constexpr int kRowBytes = D * (FP8 ? 1 : 2);
   static constexpr int kTileBytes = 16 * kRowBytes;       // 16 tokens of keys or values
   static constexpr int kStageBytes = 2 * kTileBytes;      // of one warp
-  static constexpr int kBlocks = FP8 ? 2 : 2;        // an SM
+  static constexpr int kBlocks = kAttnBlocks;             // an SM
   static constexpr int kStages = 49152 / kBlocks / kStageBytes;  // 48 KB of a warp's place in flight
   static constexpr int kNT = D / 8;                       // output tiles of 8 columns
   static constexpr int kSmem = kWarps * kStages * kStageBytes + kNT * 32 * 16;

@@ -105,6 +105,9 @@ struct AttnParams {
   int* counters;  // [blocks] zeros, left zero
   void* parts;    // [blocks][2] parts of split items
 };
+// Blocks an SM at most, and counters and parts of an item that a block can share
+// (the tiles kernel: two tiles an item).
+constexpr int kAttnBlocks = 2, kAttnTiles = 2;
 // Bytes of counters and of parts for any call on a device of num_sms SMs.
 size_t attn_counter_bytes(int num_sms);
 size_t attn_part_bytes(int num_sms, int head_dim);
