@@ -54,16 +54,6 @@ __device__ __forceinline__ uint4 load8(const T* row, int c, int k) {
     if (8 * c + i < k) w[i / 2] |= (uint32_t)h[8 * c + i] << (16 * (i & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <typename T>
-__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = Act<T>::unpack(w[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
 
 // One block a row.  A thread keeps up to 32 elements (four 16-byte loads) as
 // they come, so a row of up to 32 x threads elements is read once (a longer

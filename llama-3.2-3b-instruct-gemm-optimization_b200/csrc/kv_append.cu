@@ -51,17 +51,6 @@ __device__ __forceinline__ uint2 e4m3_quotients(const float* v, float s, float b
   return e4m3_divided(make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]), s);
 }
 
-// 16 bytes of a head.
-template <typename T>
-__device__ __forceinline__ void unpack8(uint4 v, float* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = Act<T>::unpack(w[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float* f) {
   return make_uint4(Act<T>::pack(f[0], f[1]), Act<T>::pack(f[2], f[3]), Act<T>::pack(f[4], f[5]),

@@ -81,6 +81,18 @@ struct Act<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 };
 
+// 16 bytes of activations, widened.
+template <typename T>
+__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = Act<T>::unpack(w[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+
 // One sequence's rows and cached length, clamped to what the buffers hold.
 struct SeqSpan {
   int first, n;  // its rows are first .. first + n - 1
@@ -226,7 +238,7 @@ struct AttnShare {
 // The unit that block c's range begins with.
 __host__ __device__ __forceinline__ long long attn_begin(const AttnShare& s, int c) { return mul_div(s.total, c, s.blocks); }
 
-// Sums the list (all threads; sh: blockDim.x + 1 words) and finds the block's
+// Sums the list (all threads; sh: a word a warp, two at least) and finds the block's
 // range.  At least `least` units a block, so that short work is not cut finer
 // than the joining of its pieces is worth; BY_LENGTH: one, where no sequence's
 // items are longer than four units (a block that takes several short items has
