@@ -480,7 +480,8 @@ b2g_status b2g_i8_enqueue(const b2g_i8_op* op, const b2g_i8_args* args, b2g_stre
  * E4M3 caches hold value / scale[head] (scale NULL: 1), saturated.
  * New tokens: the rows q_start[b] .. q_start[b + 1] - 1 belong to sequence
  * b, whose last row is its token seq_lens[b] - 1 (seq_lens counts them);
- * rows behind q_start[batch] are neither read nor written.
+ * rows behind q_start[batch] are not written, and what they hold does not
+ * matter.
  * A token whose page is not in 0..num_pages-1, or that lies past
  * max_pages * page_size, is not written and not seen, and sets the device
  * error word (b2g_device_error, code 6); a row before the start of its
