@@ -140,6 +140,47 @@ def test_prompts_then_decode_steps(b2g, cuda, cache):
         assert float((h.double() - want).norm() / (want - base).norm()) <= tol
 
 
+@pytest.mark.parametrize("cache", ["bf16", "fp8_e4m3"])
+def test_prompts_and_decode_rows_in_one_call(b2g, cuda, cache):
+    """bf16, calls that hold prompts, decode rows or both, a sequence without a row
+    among them.  Roundings between the operators are 2^-8 where fp16's are 2^-11: a
+    value moves by half a code at most and 0.08 on average, so eight codes in a
+    hundred fall to their neighbour, 0.28 codes rms of about 40: 7e-3 a product,
+    with the 2^-8 of q, k, v and of the probabilities under 4e-2 of an update; h
+    itself is rounded once.  8-bit keys and values: 6e-2 as above, sqrt of the
+    squares' sum."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+
+    def rand(*shape, scale=1.0):
+        return (torch.randn(*shape, device="cuda", generator=g) * scale).bfloat16()
+
+    wqkv = b2g.quantize_i8_weights(rand((HQ + 2 * HKV) * D, HIDDEN, scale=HIDDEN ** -0.5), "NK")
+    wo = b2g.quantize_i8_weights(rand(HQ * D, HIDDEN, scale=(HQ * D) ** -0.5), "KN")
+    gamma = 1 + rand(HIDDEN, scale=0.1)
+    freq = (10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) * 2 / D)).float().cuda()
+    dq = [w[0].double() * w[1].double()[:, None] for w in (wqkv, wo)]
+    block = b2g.AttentionBlock(HIDDEN, HQ, HKV, D, max_rows=256, max_batch=4, wqkv=wqkv, wo=wo, inv_freq=freq,
+                               gamma=gamma, dtype="bf16", cache_dtype=cache)
+    pool = 64
+    kind = torch.bfloat16 if cache == "bf16" else torch.float8_e4m3fn
+    paged = b2g.PagedCache(*(torch.zeros(pool, PAGE, HKV, D, device="cuda").to(kind) for _ in range(2)))
+    table = torch.randperm(pool, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(4, 16).cuda()
+    ws = block.workspace()
+    tol = 4e-2 if cache == "bf16" else 7.2e-2
+    seqs = [(torch.zeros(0, HKV, D, dtype=torch.float64, device="cuda"),) * 2 for _ in range(4)]
+    for new in ([90, 3, 40, 0], [1, 60, 1, 20], [1, 1, 0, 100], [1, 1, 1, 1]):
+        h = rand(sum(new) + 2, HIDDEN)  # two rows behind the last sequence
+        base = h[:sum(new)].double()
+        want = layer(base, new, seqs, *dq, gamma.double(), freq)
+        starts = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+        lens = torch.tensor([k.shape[0] for k, _ in seqs], dtype=torch.int32, device="cuda")
+        block.enqueue(h, paged, starts, lens, table, ws, max_q=max(new))
+        torch.cuda.synchronize()
+        assert b2g.device_error() == 0
+        off = h[:sum(new)].double() - want
+        assert float(off.norm()) <= tol * float((want - base).norm()) + 2.0 ** -8 * float(want.norm())
+
+
 def test_out_over_q(b2g, cuda):
     """AttnOp's out may be q itself, split items among them."""
     from attn_reference import attention, make_batch
