@@ -687,7 +687,8 @@ class I8Op:
 
     def enqueue(self, x, wq, sw, y=None, workspace=None, residual=None, gamma=None, rms_eps: float = 1e-5,
                 stream=None):
-        """y of 16-bit rows x [m, K], quantised (and normalised) on the way."""
+        """y of 16-bit rows x [m, K], quantised (and normalised) on the way.  Without
+        a workspace one is made and cleared for this call."""
         device, m = x.device, x.shape[0]
         index, raw = _launch(stream, device)
         ldx = _matrix(x, index, self._type, (m, self.K), 8, "x")
@@ -843,7 +844,8 @@ class AttnOp:
 
         max_q: the most new tokens of one sequence (None: unknown), a hint that
         picks the kernel.  scale: default 1 / sqrt(dim).  window: a token sees
-        the last `window` positions, its own among them (0: all).
+        the last `window` positions, its own among them (0: all).  Without a
+        workspace one is made and cleared for this call.
         """
         import torch
         rows, device = q.shape[0], q.device

@@ -26,10 +26,12 @@
 // barrier of their own: the next item's S is issued without a word from the
 // softmax warps, and on s_full its phase could end before a warp that stood
 // still had seen theirs.
-// Three chunks of up to 2048 tokens at up to 6000, 32 heads on 8, bf16: 388 us in
-// a short run, 0.91 PFLOP/s (436 in a long one at the power limit);
-// the softmax warps take 2000 clocks for 64 columns of both tiles, of which
-// the exponentials are 1024.
+// Three chunks of up to 2048 tokens at up to 6000, 32 heads on 8, bf16: 395 us in
+// a short run, 0.89 PFLOP/s (442 in a long one at the power limit); over an 8-bit
+// cache 467.  The softmax warps take 2000 clocks for 64 columns of both tiles, of
+// which the exponentials are 1024.  Of issue slots 40% are used, of the tensor
+// pipe's time 40%, of the special-function unit's 45%; registers are spilled, but
+// outside the loop (230 spill loads of a scheduler's warps in a launch).
 // Every wait is bounded.  After one has run out a products' warp is done; a thread
 // of the others goes through the remaining steps without waiting, so that their
 // barriers still meet (the loads without issuing or announcing anything, which a

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(1024) quantize_weights_kernel(const T* __restr
 // which moves two thirds of the bytes a product from L2 (what bounds the narrow
 // one: 240 clocks an MMA of 128 x 256 where the tensor cores need 128), but
 // fills tensor memory with one accumulator, drained by eight warps between
-// tiles.  4096 x 8192 x 8192: 191 us in a loop (2.9 POP/s, 0.87 of the rate that
+// tiles.  4096 x 8192 x 8192: 192 us in a loop (2.9 POP/s, 0.86 of the rate that
 // the bf16 peak implies), 247 in narrow tiles.
 // Work is cut in one of three ways (i8_plan).  Whole tiles, in turn.  A
 // cluster of 2, 4 or 8 CTAs a tile, where that many fit: each takes a part of K
